@@ -408,7 +408,7 @@ def _plain_verify(st):
             r = w
         w = torch.where((rejected & (r.sum(-1) > 0))[:, None], r, w)
         cum = w.cumsum(-1)
-        tok = (cum <= st["u"].double()[last][:, None] * cum[:, -1:]).sum(-1)
+        tok = (cum <= st["u"].double()[off + k][:, None] * cum[:, -1:]).sum(-1)
         tok = torch.minimum(tok, _argmax((w > 0).int()))
     seq = torch.repeat_interleave(torch.arange(S, device="cuda"), count, output_size=T)
     j = torch.arange(T, device="cuda") - off[seq]
@@ -522,8 +522,8 @@ def _exact_verify(case, i, new):
                 got.append(best)
                 break
             p = torch.softmax(x / case["temp"], 0)
-            u = float(i["u"][off + r])
             if r < n - 1:
+                u = float(i["u"][off + r])
                 d = int(i["tokens"][off + r + 1])
                 q = None if i["probs"] is None else i["probs"][off - s + r].double()
                 if u * (1.0 if q is None else float(q[d])) < float(p[d]):
@@ -537,7 +537,7 @@ def _exact_verify(case, i, new):
                     rest = torch.clamp(p - q, min=0.0)
                 p = rest if float(rest.sum()) > 0 else p
             total = torch.cumsum(p, 0)
-            above = (total > u * float(total[-1])).nonzero()
+            above = (total > float(i["u"][off + n - 1]) * float(total[-1])).nonzero()
             got.append(int(above[0]) if above.numel() else int((p > 0).nonzero()[-1]))
             break
         accepted.append(a)
