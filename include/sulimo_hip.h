@@ -48,6 +48,7 @@ extern "C" {
 
 typedef struct sulimo_hip_ctx sulimo_hip_ctx;
 typedef struct sulimo_hip_buffer sulimo_hip_buffer;
+typedef struct sulimo_hip_seq_batch sulimo_hip_seq_batch;
 
 /* OclDeviceInfo (crates/sulimo-ocl/src/probe.rs:9-34), HIP fields. */
 typedef struct {
@@ -340,6 +341,89 @@ int32_t sulimo_hip_kv_window_download(sulimo_hip_ctx *ctx, const sulimo_hip_kv_c
                                       int32_t *pad, int32_t *v_row_stride);
 int32_t sulimo_hip_rope_table(sulimo_hip_ctx *ctx, size_t rope_dim, float freq_base, size_t start_pos,
                               size_t n, sulimo_hip_buffer *table);
+
+/* ---- a step of several sequences over a paged Q8_0 cache (no counterpart in the
+ * reference, whose engine runs one sequence, crates/sulimo-engine/src/engine.rs:152-422) ----
+ *
+ * Each step runs a batch of sequences: sequence s has start_pos[s] positions in the cache
+ * and n_new[s] new tokens, at positions start_pos[s] .. start_pos[s] + n_new[s] - 1. The new
+ * rows of all sequences lie one behind the other in every buffer of the step ([rows][...],
+ * rows = the sum of n_new); a buffer may be longer, what lies behind the last row is
+ * neither read nor written. A cache buffer holds n_pages pages of page_size positions, a
+ * position's row being the ring's (head_count_kv * head_dim / 32 blocks of 34 bytes), one
+ * buffer for keys and one for values of a layer; position p of sequence s is row p % page_size
+ * of page page_table[s][p / page_size]. A batch serves every layer of its step.
+ *
+ * The calls are asynchronous on the context's stream. A batch is used with the context it was
+ * made with, by one thread at a time; it keeps device copies of its arrays and the workspace
+ * of its calls. Buffers must be on the context's device. */
+
+/* Head layout (head_dim 64 or 128, head_count % head_count_kv == 0), window (a query sees
+ * its own and the window - 1 positions before it; 0: all before it) and cache shape of a
+ * batch. All zero: a batch for sulimo_hip_enqueue_verify_drafts only; page_size and n_pages
+ * zero: no cache. page_size is any positive count, n_pages * page_size < 2^31. */
+int32_t sulimo_hip_seq_batch_create(sulimo_hip_ctx *ctx, size_t head_count, size_t head_count_kv, size_t head_dim,
+                                    size_t window, size_t page_size, size_t n_pages, sulimo_hip_seq_batch **out);
+/* NULL is a no-op. Waits for queued work that uses the batch. */
+int32_t sulimo_hip_seq_batch_release(sulimo_hip_seq_batch *batch);
+/* The sequences of the next calls (work already queued keeps the ones it was queued with).
+ * n_new and start_pos [n_seqs] (start_pos NULL: all zero; n_new may be zero), page_table
+ * [n_seqs][max_pages], of which the first ceil((start_pos + n_new) / page_size) entries of a
+ * sequence are read (NULL: the step uses no cache). Every one of them must be < n_pages, and
+ * a page that receives new positions must stand nowhere else in the batch (pages that are
+ * only read may be shared); else INVALID_ARGUMENT, and the batch keeps what it had. The
+ * arrays are copied. */
+int32_t sulimo_hip_seq_batch_set(sulimo_hip_seq_batch *batch, size_t n_seqs, const uint32_t *n_new,
+                                 const uint32_t *start_pos, const uint32_t *page_table, size_t max_pages);
+/* Quantizes k and v, f16 [rows][head_count_kv * head_dim], into the pages of the new
+ * positions, bytes as sulimo_hip_enqueue_kv_store writes them. k_values, v_values (f16, as k
+ * and v; each may be NULL) receive f16(code * scale), what the cache now stands for: keys and
+ * values for sulimo_hip_enqueue_attention_packed that agree with the cache. */
+int32_t sulimo_hip_enqueue_kv_store_paged(sulimo_hip_ctx *ctx, const sulimo_hip_seq_batch *batch,
+                                          const sulimo_hip_buffer *k, const sulimo_hip_buffer *v,
+                                          sulimo_hip_buffer *k_cache, sulimo_hip_buffer *v_cache,
+                                          sulimo_hip_buffer *k_values, sulimo_hip_buffer *v_values);
+/* Reads positions 0 .. start_pos + n_new - 1 of every sequence back, f16(code * scale):
+ * k_out, v_out f16 [sum of start_pos + n_new][head_count_kv * head_dim], sequence after
+ * sequence. */
+int32_t sulimo_hip_enqueue_kv_load_paged(sulimo_hip_ctx *ctx, sulimo_hip_seq_batch *batch,
+                                         const sulimo_hip_buffer *k_cache, const sulimo_hip_buffer *v_cache,
+                                         sulimo_hip_buffer *k_out, sulimo_hip_buffer *v_out);
+/* Causal GQA attention of the new rows over the paged cache (their own keys and values
+ * stored before, sulimo_hip_enqueue_kv_store_paged): q, out f16 [rows][head_count][head_dim];
+ * scores scaled by 1/sqrt(head_dim), softmax and sums in f32. */
+int32_t sulimo_hip_enqueue_attention_paged(sulimo_hip_ctx *ctx, sulimo_hip_seq_batch *batch,
+                                           const sulimo_hip_buffer *q, const sulimo_hip_buffer *k_cache,
+                                           const sulimo_hip_buffer *v_cache, sulimo_hip_buffer *out);
+/* The same for whole prompts (every start_pos zero) with their keys and values in hand:
+ * k, v f16 [rows][head_count_kv][head_dim]. The batch needs no cache. */
+int32_t sulimo_hip_enqueue_attention_packed(sulimo_hip_ctx *ctx, sulimo_hip_seq_batch *batch,
+                                            const sulimo_hip_buffer *q, const sulimo_hip_buffer *k,
+                                            const sulimo_hip_buffer *v, sulimo_hip_buffer *out);
+/* Checks drafted tokens against the target model's probabilities. The step ran each
+ * sequence's last token and its n_new - 1 drafts: tokens int32 [rows] are those inputs,
+ * logits f32 [rows][vocab] the target's answers (execute_prefill_ubatch_ex's logits_all), so
+ * row i judges token i + 1. With p = softmax(logits / temperature) of the row, q the
+ * distribution the draft was drawn from (draft_probs f32 [rows - n_seqs][vocab], one row per
+ * draft, sequence after sequence; NULL: each draft was certain, q = 1 at its token) and u
+ * = uniforms[row] (f32 [rows], in [0, 1)), drafts are accepted in order while u q(d) < p(d).
+ * The first that is not is replaced by a token of max(p - q, 0) normalized (of p if nothing is
+ * left), and behind accepted drafts only comes a token of p of the last row: the lowest
+ * token whose running sum exceeds the sequence's last uniform times the total (the uniforms
+ * of a sequence's other rows judge its drafts). temperature 0: p is 1 at the row's
+ * greatest logit (the highest index of equal ones, as argmax_all), draft_probs and uniforms
+ * are not read. Sums and probabilities are f64.
+ * accepted int32 [n_seqs] receives the number of accepted drafts a, answer int32 [rows] the
+ * sequence's a accepted drafts, the token chosen behind them, and -1 in its other rows.
+ * A NaN logit counts as -infinity; a row without any logit above -infinity accepts nothing and
+ * answers -1. A drafted token outside [0, vocab) is not accepted. A draft probability that
+ * is not above zero counts as zero (and rejects nothing), a uniform below zero or NaN as zero.
+ * Every n_new must be at least 1. */
+int32_t sulimo_hip_enqueue_verify_drafts(sulimo_hip_ctx *ctx, sulimo_hip_seq_batch *batch,
+                                         const sulimo_hip_buffer *logits, const sulimo_hip_buffer *tokens,
+                                         const sulimo_hip_buffer *draft_probs, const sulimo_hip_buffer *uniforms,
+                                         size_t vocab, float temperature, sulimo_hip_buffer *accepted,
+                                         sulimo_hip_buffer *answer);
 
 /* ---- timing (the queue's CL_QUEUE_PROFILING_ENABLE, program.rs:145-153) ---- */
 /* Per kernel class GPU time of execute_prefill_ubatch launches while profiling is on,

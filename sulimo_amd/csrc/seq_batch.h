@@ -1,0 +1,66 @@
+// seq_batch.h - the batch handle of a step, and what its kernels take.
+#pragma once
+
+#include "common.h"
+#include "seq_plan.h"
+
+namespace sulimo {
+// A grown-on-demand device array that the calls of one context fill in stream order.
+struct StepArray {
+  void *dev = nullptr;
+  size_t bytes = 0;
+};
+}  // namespace sulimo
+
+struct sulimo_hip_seq_batch {
+  sulimo_hip_ctx *ctx = nullptr;
+  int device = 0;
+  sulimo::SeqShape g;
+  sulimo::Seqs q;
+  sulimo::SeqBlob at;  // where the parts are in `seqs`
+  sulimo::StepArray seqs;
+  // position tiles of kv_load_paged, built by its first call after a set
+  sulimo::StepArray load_tiles;
+  int n_load_tiles = 0;
+  bool load_ready = false;
+};
+
+namespace sulimo {
+
+// Device pointers of a batch's sequences.
+struct SeqView {
+  const int32_t *off, *start, *page_off, *row_seq, *row_slot, *pages;
+  int n_seqs, rows, page_size, window;
+};
+SeqView seq_view(const sulimo_hip_seq_batch *b);
+
+// Grows a to at least `bytes` (after the context's queued work, before its next).
+int32_t step_array(sulimo_hip_seq_batch *b, StepArray *a, size_t bytes);
+
+// Kernel launchers of a step's operators.
+int32_t launch_kv_store_paged(const SeqView &v, int width, const uint16_t *k, const uint16_t *vv, uint8_t *k_cache,
+                              uint8_t *v_cache, uint16_t *k_values, uint16_t *v_values, hipStream_t s);
+int32_t launch_kv_load_paged(const LoadTile *tiles, int n_tiles, const int32_t *pages, int page_size, int width,
+                             const uint8_t *k_cache, const uint8_t *v_cache, uint16_t *k_out, uint16_t *v_out,
+                             hipStream_t s);
+
+// Attention of the batch's new rows: over the paged Q8_0 cache (k_cache, v_cache bytes), or
+// over the rows' own f16 keys and values.
+int32_t attention_paged(sulimo_hip_seq_batch *b, const uint16_t *q, const uint8_t *k_cache, const uint8_t *v_cache,
+                        uint16_t *out);
+int32_t attention_packed(sulimo_hip_seq_batch *b, const uint16_t *q, const uint16_t *k, const uint16_t *v,
+                         uint16_t *out);
+
+struct VerifyArgs {
+  const float *logits;       // [rows][vocab]
+  const int32_t *tokens;     // [rows]
+  const float *draft_probs;  // [rows - n_seqs][vocab], or null: each draft was certain
+  const float *uniforms;     // [rows]; not read at temperature 0
+  int vocab;
+  double temperature;
+  int32_t *accepted;  // [n_seqs]
+  int32_t *answer;    // [rows]
+};
+int32_t verify_drafts(sulimo_hip_seq_batch *b, const VerifyArgs &a);
+
+}  // namespace sulimo

@@ -179,6 +179,14 @@ def _declare(L):
         "sulimo_hip_kv_window_download": (I32, [P, C.POINTER(KvCacheC), I32, P, SZ, C.POINTER(SZ),
                                                 C.POINTER(C.c_int64), C.POINTER(I32), C.POINTER(I32)]),
         "sulimo_hip_rope_table": (I32, [P, SZ, F, SZ, SZ, P]),
+        "sulimo_hip_seq_batch_create": (I32, [P, SZ, SZ, SZ, SZ, SZ, SZ, C.POINTER(P)]),
+        "sulimo_hip_seq_batch_release": (I32, [P]),
+        "sulimo_hip_seq_batch_set": (I32, [P, SZ, P, P, P, SZ]),
+        "sulimo_hip_enqueue_kv_store_paged": (I32, [P] * 8),
+        "sulimo_hip_enqueue_kv_load_paged": (I32, [P] * 6),
+        "sulimo_hip_enqueue_attention_paged": (I32, [P] * 6),
+        "sulimo_hip_enqueue_attention_packed": (I32, [P] * 6),
+        "sulimo_hip_enqueue_verify_drafts": (I32, [P, P, P, P, P, P, SZ, F, P, P]),
         "sulimo_hip_set_profiling": (I32, [P, I32]),
         "sulimo_hip_set_graph_replay": (I32, [P, I32]),
         "sulimo_hip_get_graph_replay_counts": (I32, [P, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
@@ -407,6 +415,88 @@ def embed_tokens(ctx, embd_scales, embd_quants, tokens: np.ndarray, embd, vocab,
     t = np.ascontiguousarray(tokens, dtype=np.uint32)
     _check(lib().sulimo_hip_embed_tokens(ctx.handle, _h(embd_scales), _h(embd_quants),
                                          t.ctypes.data_as(C.c_void_p), t.size, embd, vocab, _h(x)))
+
+
+# ---- a step of several sequences over a paged Q8_0 cache ----
+
+def _u32(a, shape):
+    """A C-contiguous uint32 array of the shape; values that uint32 cannot hold raise."""
+    a = np.asarray(a)
+    if a.size == 0:
+        a = a.astype(np.uint32)
+    if a.dtype.kind not in "iu" or (a.size and (a.min() < 0 or a.max() > 0xFFFFFFFF)):
+        raise ValueError("lengths, positions and pages are whole numbers in [0, 2**32)")
+    if a.shape != shape:
+        raise ValueError(f"expected an array of shape {shape}, got {a.shape}")
+    return np.ascontiguousarray(a, dtype=np.uint32)
+
+
+class SeqBatch:
+    """The sequences of a step (sulimo_hip_seq_batch): head layout, attention window (0: none)
+    and the cache's pages; ``set`` names the sequences of the next calls."""
+
+    def __init__(self, ctx: HipContext, n_head: int = 0, n_head_kv: int = 0, head_dim: int = 0, window: int = 0,
+                 page_size: int = 0, n_pages: int = 0):
+        self.handle = C.c_void_p()
+        self.ctx = ctx
+        h = C.c_void_p()
+        _check(lib().sulimo_hip_seq_batch_create(ctx.handle, n_head, n_head_kv, head_dim, window, page_size, n_pages,
+                                                 C.byref(h)))
+        self.handle = h
+
+    def set(self, n_new, start_pos=None, page_table=None):
+        """n_new, start_pos (None: all zero): one whole number per sequence; page_table
+        [n_seqs][pages] (None: the step uses no cache)."""
+        n = len(n_new)
+        new = _u32(n_new, (n,))
+        start = _u32(start_pos, (n,)) if start_pos is not None else None
+        table, width = None, 0
+        if page_table is not None:
+            width = np.asarray(page_table).shape[1] if np.asarray(page_table).ndim == 2 else 0
+            table = _u32(page_table, (n, width))
+        ptr = [a.ctypes.data_as(C.c_void_p) if a is not None else None for a in (new, start, table)]
+        _check(lib().sulimo_hip_seq_batch_set(self.handle, n, *ptr, width))
+
+    def release(self):
+        if self.handle:
+            _check(lib().sulimo_hip_seq_batch_release(self.handle))
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            if self.handle and _lib is not None:
+                _lib.sulimo_hip_seq_batch_release(self.handle)
+                self.handle = C.c_void_p()
+        except Exception:
+            pass
+
+
+def enqueue_kv_store_paged(ctx, batch, k, v, k_cache, v_cache, k_values=None, v_values=None):
+    """New keys and values into their pages; k_values / v_values take what the cache then stands for."""
+    _check(lib().sulimo_hip_enqueue_kv_store_paged(ctx.handle, _h(batch), _h(k), _h(v), _h(k_cache), _h(v_cache),
+                                                   _h(k_values), _h(v_values)))
+
+
+def enqueue_kv_load_paged(ctx, batch, k_cache, v_cache, k_out, v_out):
+    """Every position of the batch's sequences as f16 rows, sequence after sequence."""
+    _check(lib().sulimo_hip_enqueue_kv_load_paged(ctx.handle, _h(batch), _h(k_cache), _h(v_cache), _h(k_out),
+                                                  _h(v_out)))
+
+
+def enqueue_attention_paged(ctx, batch, q, k_cache, v_cache, out):
+    """Causal GQA attention of the new rows over the paged cache."""
+    _check(lib().sulimo_hip_enqueue_attention_paged(ctx.handle, _h(batch), _h(q), _h(k_cache), _h(v_cache), _h(out)))
+
+
+def enqueue_attention_packed(ctx, batch, q, k, v, out):
+    """Causal GQA attention of whole prompts with their f16 keys and values in hand."""
+    _check(lib().sulimo_hip_enqueue_attention_packed(ctx.handle, _h(batch), _h(q), _h(k), _h(v), _h(out)))
+
+
+def enqueue_verify_drafts(ctx, batch, logits, tokens, draft_probs, uniforms, vocab, temperature, accepted, answer):
+    """Drafted tokens against the target's probabilities (draft_probs None: each was certain)."""
+    _check(lib().sulimo_hip_enqueue_verify_drafts(ctx.handle, _h(batch), _h(logits), _h(tokens), _h(draft_probs),
+                                                  _h(uniforms), vocab, temperature, _h(accepted), _h(answer)))
 
 
 # ---- whole-model device state (OclEngineState, crates/sulimo-engine/src/scheduler.rs:62-244) ----

@@ -1,0 +1,164 @@
+"""CPU: the checks of a step's sequences and what the kernels read of them
+(sulimo_amd/csrc/seq_plan.h, compiled here), and the refusals of the calls that need no device."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
+import numpy as np
+import pytest
+
+from sulimo_amd import hip
+from tests import step_reference as R
+
+CSRC = os.path.join(os.path.dirname(hip.__file__), "csrc")
+
+SOURCE = r'''
+#include "seq_plan.h"
+#include <string.h>
+using namespace sulimo;
+static std::string why;
+extern "C" const char *shape_error(size_t h, size_t hk, size_t d, size_t w, size_t p, size_t n) {
+  why = check_seq_shape(h, hk, d, w, p, n);
+  return why.c_str();
+}
+// q: what an earlier set left; the blob and the tiles go to out, their sizes to sizes
+extern "C" const char *plan(int heads, int page, int pages, size_t n, const uint32_t *nn, const uint32_t *st,
+                            const uint32_t *table, size_t width, int32_t *out, size_t *sizes) {
+  SeqShape g{heads, 1, 64, 0, page, pages};
+  Seqs q;
+  q.rows = 77;
+  why = plan_seqs(g, n, nn, st, table, width, &q);
+  if (!why.empty()) {
+    if (q.rows != 77) why = "a refused set changed the batch";
+    return why.c_str();
+  }
+  const SeqBlob b = seq_blob(g, q);
+  memcpy(out, b.data.data(), b.data.size() * 4);
+  const size_t s[] = {b.start, b.page_off, b.row_seq, b.row_slot, b.pages, b.data.size(), (size_t)q.rows, (size_t)q.positions};
+  memcpy(sizes, s, sizeof s);
+  int32_t *t = out + b.data.size();
+  size_t k = 0;
+  for (const LoadTile &l : load_tiles(q)) {
+    t[4 * k] = l.page_off; t[4 * k + 1] = l.pos; t[4 * k + 2] = l.out_row; t[4 * k++ + 3] = l.count;
+  }
+  sizes[8] = k;
+  return "";
+}
+'''
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    if shutil.which("g++") is None:
+        pytest.skip("g++ is not installed")
+    d = tmp_path_factory.mktemp("seq")
+    (d / "s.cpp").write_text(SOURCE)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-I", CSRC, str(d / "s.cpp"), "-o",
+                    str(d / "s.so")], check=True)
+    L = C.CDLL(str(d / "s.so"))
+    L.shape_error.restype = L.plan.restype = C.c_char_p
+    L.shape_error.argtypes = [C.c_size_t] * 6
+    L.plan.argtypes = [C.c_int] * 3 + [C.c_size_t] + [C.c_void_p] * 3 + [C.c_size_t] + [C.c_void_p] * 2
+    return L
+
+
+def plan(lib, n_new, start=None, table=None, page=0, pages=0, heads=4, n=None):
+    nn = np.asarray(n_new, np.uint32)
+    st = None if start is None else np.asarray(start, np.uint32)
+    tb = None if table is None else np.ascontiguousarray(table, np.uint32)
+    out, sizes = np.zeros(1 << 20, np.int32), np.zeros(9, np.uint64)
+    p = [None if a is None else a.ctypes.data for a in (nn, st, tb)]
+    why = lib.plan(heads, page, pages, len(nn) if n is None else n, *p, 0 if tb is None else tb.shape[1], out.ctypes.data,
+                   sizes.ctypes.data).decode()
+    return why, out, [int(x) for x in sizes]
+
+
+@pytest.mark.parametrize("page,start,new", [(1, [0, 3, 5], [2, 0, 1]), (7, [13, 0, 6], [1, 20, 1]), (64, [64, 63, 0], [64, 2, 0]),
+                                            (256, [1000], [300])])
+def test_rows_slots_and_tiles(lib, page, start, new):
+    need = [-(-(a + b) // page) for a, b in zip(start, new)]
+    pages = sum(need) + 3
+    order = np.random.default_rng(page).permutation(pages)
+    table = np.full((len(new), max(need) + 1), 4000000000, np.uint32)  # entries behind the last are not read
+    at = 0
+    for s, k in enumerate(need):
+        table[s, :k] = order[at:at + k]
+        at += k
+    why, out, z = plan(lib, new, start, table, page, pages)
+    assert why == ""
+    n, rows = len(new), sum(new)
+    assert z[6] == rows and z[7] == rows + sum(start)
+    off = np.concatenate([[0], np.cumsum(new)])
+    assert np.array_equal(out[:n + 1], off) and np.array_equal(out[z[0]:z[0] + n], start)
+    assert np.array_equal(out[z[2]:z[2] + rows], np.repeat(np.arange(n), new))
+    slots = np.concatenate([R.slots(table[s], page, a, a + b) for s, (a, b) in enumerate(zip(start, new))])
+    assert np.array_equal(out[z[3]:z[3] + rows], slots)
+    page_off = out[z[1]:z[1] + n]
+    for s in range(n):
+        assert np.array_equal(out[z[4] + page_off[s]:z[4] + page_off[s] + need[s]], table[s, :need[s]])
+    # the load tiles cover every position once, in order, and none passes a sequence's end
+    tiles = out[z[5]:z[5] + 4 * z[8]].reshape(-1, 4)
+    want = [(page_off[s], p) for s in range(n) for p in range(start[s] + new[s])]
+    got = [(t[0], t[1] + i) for t in tiles for i in range(t[3])]
+    assert got == want
+    assert np.array_equal(tiles[:, 2], np.concatenate([[0], np.cumsum(tiles[:, 3])[:-1]]) if len(tiles) else [])
+
+
+@pytest.mark.parametrize("args,word", [
+    (dict(n_new=[1], start=[7], table=[[0, 8]], page=4, pages=8), "n_pages"),
+    (dict(n_new=[1], start=[7], table=[[9, 1]], page=4, pages=8), "n_pages"),
+    (dict(n_new=[2], start=[7], table=[[0, 1]], page=4, pages=8), "needs 3 pages"),
+    (dict(n_new=[1, 1], start=[0, 0], table=[[3], [3]], page=4, pages=8), "twice"),
+    (dict(n_new=[8], start=[0], table=[[3, 3]], page=4, pages=8), "twice"),
+    (dict(n_new=[1, 1], start=[4, 0], table=[[3, 1], [3, 0]], page=4, pages=8), "elsewhere"),
+    (dict(n_new=[1, 0], start=[0, 3], table=[[3], [3]], page=4, pages=8), "elsewhere"),
+    (dict(n_new=[1], table=[[0]], page=0, pages=0), "batch with pages"),
+    (dict(n_new=[2**31]), "too long"),
+    (dict(n_new=[1], start=[2**32 - 1]), "too long"),
+    (dict(n_new=[2**30], heads=24), "too long together"),
+    (dict(n_new=[1] * 3, start=[2**30] * 3), "too long together"),
+    (dict(n_new=[1], n=65536), "65535"),
+])
+def test_refused_sequences(lib, args, word):
+    why, _, _ = plan(lib, **args)
+    assert word in why
+
+
+def test_pages_that_are_only_read_may_be_shared(lib):
+    table = [[5, 0], [5, 1], [5, 2]]
+    why, _, _ = plan(lib, [1, 1, 0], [4, 6, 4], table, 4, 6)
+    assert why == ""
+
+
+@pytest.mark.parametrize("shape,word", [
+    ((12, 5, 128, 0, 0, 0), "multiple"), ((12, 0, 128, 0, 0, 0), "multiple"), ((0, 2, 128, 0, 0, 0), "multiple"),
+    ((2048, 2, 128, 0, 0, 0), "multiple"), ((12, 2, 96, 0, 0, 0), "64 or 128"), ((12, 2, 0, 0, 0, 0), "64 or 128"),
+    ((0, 0, 0, 5, 0, 0), "head layout"), ((0, 0, 0, 0, 16, 4), "head layout"), ((12, 2, 128, 0, 16, 0), "together"),
+    ((12, 2, 128, 0, 0, 4), "together"), ((12, 2, 128, 0, 1 << 16, 1 << 15), "2^31"), ((12, 2, 128, 1 << 31, 0, 0), "window"),
+    ((12, 2, 128, 0, 1 << 40, 1 << 40), "2^31"),
+])
+def test_refused_shapes(lib, shape, word):
+    assert word in lib.shape_error(*shape).decode()
+    h = C.c_void_p()
+    assert hip.lib().sulimo_hip_seq_batch_create(None, *shape, C.byref(h)) == hip.ERR_INVALID_ARGUMENT
+    assert word in hip.lib().sulimo_hip_last_error().decode() and not h
+
+
+def test_calls_without_a_batch_are_refused():
+    L = hip.lib()
+    h = C.c_void_p()
+    assert L.sulimo_hip_seq_batch_create(None, 12, 2, 128, 0, 0, 0, C.byref(h)) == hip.ERR_INVALID_ARGUMENT
+    assert L.sulimo_hip_seq_batch_create(None, 12, 2, 128, 0, 0, 0, None) == hip.ERR_INVALID_ARGUMENT
+    assert L.sulimo_hip_seq_batch_set(None, 0, None, None, None, 0) == hip.ERR_INVALID_ARGUMENT
+    assert L.sulimo_hip_seq_batch_release(None) == hip.OK
+    assert L.sulimo_hip_enqueue_kv_store_paged(*[None] * 8) == hip.ERR_INVALID_ARGUMENT
+    for f in (L.sulimo_hip_enqueue_kv_load_paged, L.sulimo_hip_enqueue_attention_paged, L.sulimo_hip_enqueue_attention_packed):
+        assert f(*[None] * 6) == hip.ERR_INVALID_ARGUMENT
+    assert L.sulimo_hip_enqueue_verify_drafts(*[None] * 6, 10, 1.0, None, None) == hip.ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("bad", [[-1], [2**32], [1.5], [[1]]])
+def test_lengths_that_are_no_lengths_raise(bad):
+    with pytest.raises(ValueError):
+        hip._u32(bad, (1,))
