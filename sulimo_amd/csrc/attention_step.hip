@@ -1,101 +1,130 @@
-// attention_step.hip - causal grouped attention of a step's sequences.
+// attention_step.hip - which kernels a step's attention runs, and their work lists.
 //
-// Query row t of sequence s is position P = start[s] + t and sees positions
-// max(0, P - window + 1) .. P of its own sequence (window 0: all):
-//   out = sum_p softmax_p(q . K_p / sqrt(d)) V_p
-// with K, V = code * f16(scale) of the paged Q8_0 cache, or f16 rows of the batch.
-#include <math.h>
+// A list depends on the batch's sequences only; it is built by the first call after a set and
+// serves every layer of the step. Records of split row tiles and the part of the cache that is
+// read back live in the context's workspace, whose users run one after the other.
+#include <string.h>
 
-#include "seq_batch.h"
+#include "step_attn.h"
 
 namespace sulimo {
 namespace {
 
-struct StepAttn {
-  SeqView v;
-  const _Float16 *q;  // [rows][n_head][HD]
-  _Float16 *out;
-  const uint8_t *k_cache, *v_cache;  // paged
-  const _Float16 *k, *vv;            // packed [rows][n_head_kv][HD]
-  int n_head, n_head_kv;
-};
+#define STEP_TRY(call)          \
+  do {                          \
+    const int32_t rc_ = (call); \
+    if (rc_) return rc_;        \
+  } while (0)
 
-// One wave per (row, head): 64 keys at a time, one per lane.
-template <int HD, bool PAGED>
-__global__ __launch_bounds__(64) void step_attn_simple_kernel(StepAttn a) {
-  constexpr int DL = HD / 64;  // output elements of a lane
-  __shared__ float qs[HD];
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  const int s = a.v.row_seq[row], kvh = h / (a.n_head / a.n_head_kv);
-  const int P = a.v.start[s] + row - a.v.off[s];
-  const _Float16 *q = a.q + ((size_t)row * a.n_head + h) * HD;
-  for (int i = lane; i < HD; i += 64) qs[i] = (float)q[i];
-  __syncthreads();
-  const int lo = a.v.window ? max(0, P - a.v.window + 1) : 0;
-  const int32_t *pt = a.v.pages + a.v.page_off[s];
-  const size_t width = (size_t)a.n_head_kv * HD, bytes = width / 32 * 34;
-  auto slot = [&](int p) { return (size_t)pt[p / a.v.page_size] * a.v.page_size + p % a.v.page_size; };
-  auto value = [&](const uint8_t *cache, const _Float16 *rows, size_t r, int i) {
-    if constexpr (PAGED) {
-      const uint8_t *b = cache + r * bytes + (size_t)(kvh * (HD / 32) + i / 32) * 34;
-      return (float)(int8_t)b[2 + i % 32] * (float)*reinterpret_cast<const _Float16 *>(b);
-    } else {
-      return (float)rows[r * width + kvh * HD + i];
-    }
-  };
-  float m = -INFINITY, l = 0.0f, o[DL] = {};
-  for (int p0 = lo; p0 <= P; p0 += 64) {
-    const int p = p0 + lane;
-    size_t r = 0;
-    float x = -INFINITY;
-    if (p <= P) {
-      r = PAGED ? slot(p) : (size_t)a.v.off[s] + p;
-      float acc = 0.0f;
-      for (int i = 0; i < HD; i++) acc += qs[i] * value(a.k_cache, a.k, r, i);
-      x = acc / sqrtf((float)HD);
-    }
-    float mx = x;
-    for (int e = 32; e >= 1; e >>= 1) mx = fmaxf(mx, __shfl_xor(mx, e, 64));
-    const float mn = fmaxf(m, mx);
-    const float w = expf(x - mn), al = expf(m - mn);
-    float sum = w;
-    for (int e = 32; e >= 1; e >>= 1) sum += __shfl_xor(sum, e, 64);
-    l = l * al + sum;
-    m = mn;
-    for (int e = 0; e < DL; e++) o[e] *= al;
-    const int cnt = min(64, P - p0 + 1);
-    for (int j = 0; j < cnt; j++) {
-      const float wj = __shfl(w, j, 64);
-      const size_t rj = __shfl((long)r, j, 64);
-      for (int e = 0; e < DL; e++) o[e] += wj * value(a.v_cache, a.vv, rj, lane + 64 * e);
+constexpr size_t align_up(size_t v) { return (v + 255) & ~(size_t)255; }
+
+// Rows a KV head up to which a sequence's rows read the Q8_0 cache directly.
+constexpr int kDirectRows = 128;
+
+int32_t plan(sulimo_hip_seq_batch *b, bool packed) {
+  StepPlan &p = packed ? b->packed_plan : b->paged_plan;
+  if (p.ready) return SULIMO_HIP_OK;
+  const int cus = device_cu_count(), G = b->g.n_head / b->g.n_head_kv;
+  std::vector<int> few, many;
+  for (int s = 0; s < b->q.n_seqs; s++) {
+    if (b->q.n_new[s] == 0) continue;
+    (!packed && (long)b->q.n_new[s] * G <= kDirectRows ? few : many).push_back(s);
+  }
+  const AttnPlan c = plan_attention_pieces(b->g, b->q, few, cache_split(b->g, cus));
+  const AttnPlan r = plan_attention_pieces(b->g, b->q, many, row_split(cus));
+  std::vector<SeqKv> kv(b->q.n_seqs, SeqKv{0, 0, 0});
+  std::vector<LoadTile> tiles;
+  long rows = 0;
+  for (int s : many) {
+    const int end = b->q.start[s] + b->q.n_new[s];
+    const int lo = first_seen(b->g, b->q.start[s]) / kRowKeys * kRowKeys;
+    kv[s] = packed ? SeqKv{b->q.off[s], 0, end} : SeqKv{(int32_t)rows, lo, end - lo};
+    // the kernel's offsets inside a sequence are 32-bit (a tile may start at its last row)
+    if ((size_t)(end - lo + kRowKeys) * b->g.n_head_kv * b->g.head_dim * 2 > 0xFFFFFFFFull)
+      return fail(SULIMO_HIP_ERR_INVALID_ARGUMENT,
+                  "sequence " + std::to_string(s) + " has over 4 GiB of f16 keys in sight of a long chunk");
+    if (!packed) {
+      add_load_tiles(b->q, s, lo, end, (int)rows, &tiles);
+      rows += end - lo;
     }
   }
-  for (int e = 0; e < DL; e++) a.out[((size_t)row * a.n_head + h) * HD + lane + 64 * e] = (_Float16)(o[e] / l);
+  // one array: pieces, pieces, where the keys are, load tiles, counters (zero)
+  p.n_cache = (int)c.pieces.size();
+  p.n_rows = (int)r.pieces.size();
+  p.n_tiles = (int)tiles.size();
+  p.read_rows = rows;
+  p.cache_rec = c.rec_rows;
+  p.rec_rows = c.rec_rows + r.rec_rows;
+  p.at_rows = align_up(c.pieces.size() * sizeof(AttnPiece));
+  p.at_kv = p.at_rows + align_up(r.pieces.size() * sizeof(AttnPiece));
+  p.at_tiles = p.at_kv + align_up(kv.size() * sizeof(SeqKv));
+  p.at_cache_counters = p.at_tiles + align_up(tiles.size() * sizeof(LoadTile));
+  p.at_row_counters = p.at_cache_counters + align_up((size_t)c.counters * 4);
+  std::vector<char> blob(p.at_row_counters + align_up((size_t)r.counters * 4), 0);
+  auto put = [&](size_t at, const void *src, size_t n) {
+    if (n) memcpy(blob.data() + at, src, n);
+  };
+  put(0, c.pieces.data(), c.pieces.size() * sizeof(AttnPiece));
+  put(p.at_rows, r.pieces.data(), r.pieces.size() * sizeof(AttnPiece));
+  put(p.at_kv, kv.data(), kv.size() * sizeof(SeqKv));
+  put(p.at_tiles, tiles.data(), tiles.size() * sizeof(LoadTile));
+  if (blob.empty()) blob.resize(256, 0);
+  STEP_TRY(step_array(b, &p.lists, blob.size()));
+  SULIMO_HIP_TRY(hipMemcpyAsync(p.lists.dev, blob.data(), blob.size(), hipMemcpyHostToDevice, b->ctx->stream));
+  p.ready = true;
+  return SULIMO_HIP_OK;
 }
 
-template <bool PAGED>
-int32_t run(const StepAttn &a, int hd, hipStream_t s) {
-  const dim3 grid(a.v.rows, a.n_head);
-  if (hd == 64) hipLaunchKernelGGL((step_attn_simple_kernel<64, PAGED>), grid, dim3(64), 0, s, a);
-  else hipLaunchKernelGGL((step_attn_simple_kernel<128, PAGED>), grid, dim3(64), 0, s, a);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? SULIMO_HIP_OK : hip_fail(e, "step_attn_simple_kernel launch");
+int32_t attend(sulimo_hip_seq_batch *b, StepPlan &p, const uint16_t *q, const uint8_t *k_cache, const uint8_t *v_cache,
+               const uint16_t *k, const uint16_t *v, uint16_t *out) {
+  sulimo_hip_ctx *ctx = b->ctx;
+  const size_t hd = b->g.head_dim, width = (size_t)b->g.n_head_kv * hd;
+  const size_t o_bytes = align_up(p.rec_rows * hd * 4), ml_bytes = align_up(p.rec_rows * 8);
+  const size_t kv_bytes = align_up((size_t)p.read_rows * width * 2);
+  STEP_TRY(ensure_workspace(ctx, o_bytes + ml_bytes + 2 * kv_bytes));
+  char *ws = reinterpret_cast<char *>(ctx->ws), *lists = reinterpret_cast<char *>(p.lists.dev);
+  float *rec_o = reinterpret_cast<float *>(ws);
+  float2 *rec_ml = reinterpret_cast<float2 *>(ws + o_bytes);
+  const StepAttnArgs base{seq_view(b), nullptr, 0, reinterpret_cast<const _Float16 *>(q),
+                          reinterpret_cast<_Float16 *>(out), b->g.n_head, b->g.n_head_kv, b->g.head_dim, Join{}};
+  if (p.n_cache) {
+    StepAttnArgs c = base;
+    c.pieces = reinterpret_cast<const AttnPiece *>(lists);
+    c.n_pieces = p.n_cache;
+    c.join = Join{rec_o, rec_ml, reinterpret_cast<int *>(lists + p.at_cache_counters)};
+    STEP_TRY(launch_cache_attention(c, k_cache, v_cache, ctx->stream));
+  }
+  if (p.n_rows) {
+    uint16_t *kr = reinterpret_cast<uint16_t *>(ws + o_bytes + ml_bytes);
+    uint16_t *vr = reinterpret_cast<uint16_t *>(ws + o_bytes + ml_bytes + kv_bytes);
+    if (p.n_tiles) {
+      STEP_TRY(launch_kv_load_paged(reinterpret_cast<const LoadTile *>(lists + p.at_tiles), p.n_tiles, seq_view(b).pages,
+                                    b->g.page_size, (int)width, k_cache, v_cache, kr, vr, ctx->stream));
+      k = kr;
+      v = vr;
+    }
+    StepAttnArgs r = base;
+    r.pieces = reinterpret_cast<const AttnPiece *>(lists + p.at_rows);
+    r.n_pieces = p.n_rows;
+    r.join = Join{rec_o + p.cache_rec * hd, rec_ml + p.cache_rec, reinterpret_cast<int *>(lists + p.at_row_counters)};
+    STEP_TRY(launch_row_attention(r, reinterpret_cast<const SeqKv *>(lists + p.at_kv), reinterpret_cast<const _Float16 *>(k),
+                                  reinterpret_cast<const _Float16 *>(v), ctx->stream));
+  }
+  return SULIMO_HIP_OK;
 }
 
 }  // namespace
 
 int32_t attention_paged(sulimo_hip_seq_batch *b, const uint16_t *q, const uint8_t *k_cache, const uint8_t *v_cache,
                         uint16_t *out) {
-  StepAttn a{seq_view(b), reinterpret_cast<const _Float16 *>(q), reinterpret_cast<_Float16 *>(out), k_cache, v_cache,
-             nullptr, nullptr, b->g.n_head, b->g.n_head_kv};
-  return run<true>(a, b->g.head_dim, b->ctx->stream);
+  STEP_TRY(plan(b, false));
+  return attend(b, b->paged_plan, q, k_cache, v_cache, nullptr, nullptr, out);
 }
 
 int32_t attention_packed(sulimo_hip_seq_batch *b, const uint16_t *q, const uint16_t *k, const uint16_t *v,
                          uint16_t *out) {
-  StepAttn a{seq_view(b), reinterpret_cast<const _Float16 *>(q), reinterpret_cast<_Float16 *>(out), nullptr, nullptr,
-             reinterpret_cast<const _Float16 *>(k), reinterpret_cast<const _Float16 *>(v), b->g.n_head, b->g.n_head_kv};
-  return run<false>(a, b->g.head_dim, b->ctx->stream);
+  STEP_TRY(plan(b, true));
+  return attend(b, b->packed_plan, q, nullptr, nullptr, k, v, out);
 }
 
 }  // namespace sulimo

@@ -10,6 +10,15 @@ struct StepArray {
   void *dev = nullptr;
   size_t bytes = 0;
 };
+// The work lists of a step's attention (attention_step.hip), for the paged or the packed form.
+struct StepPlan {
+  bool ready = false;
+  StepArray lists;
+  int n_cache = 0, n_rows = 0, n_tiles = 0;  // pieces over the cache, pieces over f16 rows, load tiles
+  long read_rows = 0;                        // cache rows that are read back
+  size_t cache_rec = 0, rec_rows = 0;
+  size_t at_rows = 0, at_kv = 0, at_tiles = 0, at_cache_counters = 0, at_row_counters = 0;
+};
 }  // namespace sulimo
 
 struct sulimo_hip_seq_batch {
@@ -23,6 +32,7 @@ struct sulimo_hip_seq_batch {
   sulimo::StepArray load_tiles;
   int n_load_tiles = 0;
   bool load_ready = false;
+  sulimo::StepPlan paged_plan, packed_plan;
 };
 
 namespace sulimo {

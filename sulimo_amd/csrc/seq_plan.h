@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <numeric>
 #include <string>
 #include <vector>
 
@@ -143,16 +144,131 @@ inline SeqBlob seq_blob(const SeqShape &g, const Seqs &q) {
   return b;
 }
 
+// Positions lo .. end - 1 of sequence s, to rows row .. of the output.
+inline void add_load_tiles(const Seqs &q, int s, int lo, int end, int row, std::vector<LoadTile> *t) {
+  for (int p = lo; p < end; p += kLoadTile)
+    t->push_back(LoadTile{q.page_off[s], p, row + p - lo, std::min(kLoadTile, end - p)});
+}
 inline std::vector<LoadTile> load_tiles(const Seqs &q) {
   std::vector<LoadTile> t;
   int row = 0;
   for (int s = 0; s < q.n_seqs; s++) {
     const int len = q.start[s] + q.n_new[s];
-    for (int p = 0; p < len; p += kLoadTile)
-      t.push_back(LoadTile{q.page_off[s], p, row + p, std::min(kLoadTile, len - p)});
+    add_load_tiles(q, s, 0, len, row, &t);
     row += len;
   }
   return t;
+}
+
+// ---- attention: row tiles, and how their keys are cut ----
+// A row tile is some query rows of one KV head, row r = token r / G, head kvh * G + r % G with
+// G = n_head / n_head_kv query heads a KV head. A workgroup takes `heads` KV heads of a row tile
+// and `sub` key tiles a step, for a run of key tiles: a piece. Pieces of a row tile leave
+// records that the last one to finish joins.
+struct AttnPiece {
+  int32_t seq, row0;          // row tile: rows row0 .. of the sequence's n_new * G
+  int32_t tile0, tile1;       // key tiles of this piece (tile t: positions t * key tile ..)
+  int32_t piece, n_pieces;
+  int32_t rec;                // first record row of the tile (piece p, head h, row r at rec + (p Hk + h) live + r)
+  int32_t counter;            // index of the tile's arrival counters (one per head group)
+};
+struct AttnSplit {
+  int rows;      // of a row tile
+  int key_tile;  // positions
+  int heads, sub;
+  int slots;     // workgroups that run at once
+};
+struct AttnPlan {
+  std::vector<AttnPiece> pieces;
+  int counters = 0;     // arrival counters (head groups of every split tile)
+  size_t rec_rows = 0;  // record rows, each head_dim floats and (m, l)
+};
+inline int first_seen(const SeqShape &g, int pos) { return g.window && pos >= g.window ? pos - g.window + 1 : 0; }
+
+// The row tiles of the sequences in `which`, cut so that their workgroups run in as few rounds
+// of `slots` as the uncut tiles would need: the smallest piece that keeps to that.
+inline AttnPlan plan_attention_pieces(const SeqShape &g, const Seqs &q, const std::vector<int> &which, const AttnSplit &a) {
+  AttnPlan plan;
+  const int G = g.n_head / g.n_head_kv, groups = g.n_head_kv / a.heads;
+  struct Tile {
+    int seq, row0, live, t0, t1, steps;
+  };
+  std::vector<Tile> tiles;
+  int most = 1;
+  for (int s : which) {
+    const int total = q.n_new[s] * G;
+    for (int r0 = 0; r0 < total; r0 += a.rows) {
+      const int live = std::min(a.rows, total - r0);
+      const int first = q.start[s] + r0 / G, last = q.start[s] + (r0 + live - 1) / G;
+      Tile t{s, r0, live, first_seen(g, first) / a.key_tile, last / a.key_tile + 1, 0};
+      t.steps = (t.t1 - t.t0 + a.sub - 1) / a.sub;
+      most = std::max(most, t.steps);
+      tiles.push_back(t);
+    }
+  }
+  if (tiles.empty()) return plan;
+  const long per_round = std::max(1, a.slots / groups);
+  const long limit = ((long)tiles.size() + per_round - 1) / per_round * per_round;
+  auto fits = [&](int C) {
+    long n = 0;
+    for (const Tile &t : tiles) n += (t.steps + C - 1) / C;
+    return n <= limit;
+  };
+  int C = 1;
+  for (int hi = most; C < hi;) {  // C = most fits: one piece a tile
+    const int mid = C + (hi - C) / 2;
+    if (fits(mid)) hi = mid;
+    else C = mid + 1;
+  }
+  for (const Tile &t : tiles) {
+    const int np = (t.steps + C - 1) / C;
+    AttnPiece p{t.seq, t.row0, 0, 0, 0, np, (int32_t)plan.rec_rows, plan.counters};
+    for (int i = 0; i < np; i++) {
+      p.piece = i;
+      p.tile0 = t.t0 + (int)((long)i * t.steps / np) * a.sub;
+      p.tile1 = std::min(t.t1, t.t0 + (int)((long)(i + 1) * t.steps / np) * a.sub);
+      plan.pieces.push_back(p);
+    }
+    if (np > 1) {
+      plan.counters += groups;
+      plan.rec_rows += (size_t)np * g.n_head_kv * t.live;
+    }
+  }
+  // longest first: what starts last is short
+  std::stable_sort(plan.pieces.begin(), plan.pieces.end(), [](const AttnPiece &x, const AttnPiece &y) {
+    return x.tile1 - x.tile0 > y.tile1 - y.tile0;
+  });
+  return plan;
+}
+
+// Few rows read the Q8_0 cache directly (attention_cache.hip): 8 waves, of which 8 / heads share
+// a KV head and take every (8 / heads)th key tile.
+constexpr int kCacheRows = 32, kCacheWaves = 8;
+inline int cache_heads(int n_head_kv) {  // the largest power of two up to 8 that divides
+  return n_head_kv % 8 == 0 ? 8 : n_head_kv % 4 == 0 ? 4 : n_head_kv % 2 == 0 ? 2 : 1;
+}
+inline AttnSplit cache_split(const SeqShape &g, int cus) {
+  const int heads = cache_heads(g.n_head_kv);
+  return AttnSplit{kCacheRows, g.head_dim == 128 ? 32 : 64, heads, kCacheWaves / heads, cus};
+}
+// Many rows read f16 keys and values (attention_rows.hip), the cache's read back first.
+constexpr int kRowTile = 128, kRowKeys = 64;
+inline AttnSplit row_split(int cus) { return AttnSplit{kRowTile, kRowKeys, 1, 1, 2 * cus}; }
+
+// Where a sequence's f16 keys and values lie: position p in [lo, lo + len) is row row0 + p - lo.
+struct SeqKv {
+  int32_t row0, lo, len;
+};
+
+// p / d = p * magic >> shift for every p < 2^31 (d >= 1): magic = floor(2^(31 + b) / d) + 1 with
+// 2^b >= d is off by less than 2^-b <= 1 / d of the quotient.
+struct FastDiv {
+  uint32_t magic, shift, d;
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t b = 0;
+  while ((1ull << b) < d) b++;
+  return FastDiv{(uint32_t)(((1ull << (31 + b)) / d) + 1), 31 + b, d};
 }
 
 }  // namespace sulimo

@@ -45,6 +45,25 @@ extern "C" const char *plan(int heads, int page, int pages, size_t n, const uint
   sizes[8] = k;
   return "";
 }
+// the pieces of all sequences, 8 numbers each, and their count, counters and record rows
+extern "C" void pieces(int heads, int kv_heads, int hd, int window, size_t n, const uint32_t *nn, const uint32_t *st, int rows,
+                       int key_tile, int group_heads, int sub, int slots, int32_t *out, size_t *sizes) {
+  SeqShape g{heads, kv_heads, hd, window, 0, 0};
+  Seqs q;
+  plan_seqs(g, n, nn, st, nullptr, 0, &q);
+  std::vector<int> all(n);
+  for (size_t s = 0; s < n; s++) all[s] = (int)s;
+  const AttnPlan p = plan_attention_pieces(g, q, all, AttnSplit{rows, key_tile, group_heads, sub, slots});
+  memcpy(out, p.pieces.data(), p.pieces.size() * sizeof(AttnPiece));
+  sizes[0] = p.pieces.size();
+  sizes[1] = (size_t)p.counters;
+  sizes[2] = p.rec_rows;
+}
+extern "C" uint32_t divided(uint32_t p, uint32_t d) {
+  const FastDiv f = fast_div(d);
+  return (uint32_t)(((uint64_t)p * f.magic) >> f.shift);
+}
+extern "C" int heads_of(int hk) { return cache_heads(hk); }
 '''
 
 
@@ -59,6 +78,9 @@ def lib(tmp_path_factory):
     L = C.CDLL(str(d / "s.so"))
     L.shape_error.restype = L.plan.restype = C.c_char_p
     L.shape_error.argtypes = [C.c_size_t] * 6
+    L.pieces.argtypes = [C.c_int] * 4 + [C.c_size_t] + [C.c_void_p] * 2 + [C.c_int] * 5 + [C.c_void_p] * 2
+    L.pieces.restype = None
+    L.divided.argtypes, L.divided.restype = [C.c_uint32] * 2, C.c_uint32
     L.plan.argtypes = [C.c_int] * 3 + [C.c_size_t] + [C.c_void_p] * 3 + [C.c_size_t] + [C.c_void_p] * 2
     return L
 
@@ -162,3 +184,59 @@ def test_calls_without_a_batch_are_refused():
 def test_lengths_that_are_no_lengths_raise(bad):
     with pytest.raises(ValueError):
         hip._u32(bad, (1,))
+
+
+@pytest.mark.parametrize("rows,key_tile,heads,sub", [(32, 32, 8, 1), (32, 32, 2, 4), (32, 64, 1, 8), (128, 64, 1, 1)])
+@pytest.mark.parametrize("slots", [1, 40, 256, 512])
+@pytest.mark.parametrize("window", [0, 1, 100])
+@pytest.mark.parametrize("new,start", [([1], [0]), ([1], [5000]), ([1, 0, 7, 200], [3, 9, 4000, 70]), ([1] * 300, list(range(300))),
+                                       ([2000, 31], [0, 1])])
+def test_pieces_cover_every_key_once(lib, rows, key_tile, heads, sub, slots, window, new, start):
+    H, Hk = 24, 8
+    G = H // Hk
+    nn, st = np.asarray(new, np.uint32), np.asarray(start, np.uint32)
+    out, z = np.zeros(1 << 18, np.int32), np.zeros(3, np.uint64)
+    lib.pieces(H, Hk, 128, window, len(new), nn.ctypes.data, st.ctypes.data, rows, key_tile, heads, sub, slots, out.ctypes.data,
+               z.ctypes.data)
+    n, counters, rec_rows = (int(x) for x in z)
+    p = out[:8 * n].reshape(n, 8)
+    assert np.all(np.diff(p[:, 3] - p[:, 2]) <= 0)  # longest first
+    tiles = {}
+    for seq, row0, t0, t1, piece, np_, rec, counter in p:
+        assert t0 < t1
+        tiles.setdefault((seq, row0), []).append((piece, t0, t1, np_, rec, counter))
+    want = {(s, r) for s in range(len(new)) for r in range(0, new[s] * G, rows)}
+    assert set(tiles) == want
+    used, recs = set(), []
+    for (s, r0), ps in tiles.items():
+        ps.sort()
+        live = min(rows, new[s] * G - r0)
+        first, last = start[s] + r0 // G, start[s] + (r0 + live - 1) // G
+        lo = max(0, first - window + 1) if window else 0
+        assert [x[0] for x in ps] == list(range(ps[0][3])) and all(x[3:] == ps[0][3:] for x in ps)
+        assert ps[0][1] == lo // key_tile and ps[-1][2] == last // key_tile + 1
+        assert all(a[2] == b[1] for a, b in zip(ps, ps[1:]))
+        if len(ps) > 1:
+            groups = Hk // heads
+            mine = set(range(ps[0][5], ps[0][5] + groups))
+            assert not mine & used and max(mine) < counters
+            used |= mine
+            recs.append((ps[0][4], ps[0][4] + len(ps) * Hk * live))
+    recs.sort()
+    assert all(a[1] <= b[0] for a, b in zip(recs, recs[1:])) and (not recs or recs[-1][1] <= rec_rows)
+    per_round = max(1, slots // (Hk // heads))
+    assert n <= -(-len(want) // per_round) * per_round
+
+
+def test_division_by_the_page_size(lib):
+    rng = np.random.default_rng(0)
+    for d in [1, 2, 3, 5, 7, 16, 48, 64, 100, 255, 256, 1000, 65535, 65536, 10**6 + 3, 2**30, 2**31 - 1]:
+        for p in [0, 1, d - 1, d, d + 1, 2 * d - 1, 2 * d, 2**31 - 1, 2**31 - 2] + [int(x) for x in rng.integers(0, 2**31, 200)]:
+            if p < 2**31:
+                assert lib.divided(p, d) == p // d, (p, d)
+
+
+def test_heads_of_a_workgroup(lib):
+    for hk in range(1, 65):
+        h = lib.heads_of(hk)
+        assert h in (1, 2, 4, 8) and hk % h == 0 and (h == 8 or hk % (2 * h) != 0)
