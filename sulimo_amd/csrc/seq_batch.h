@@ -33,6 +33,7 @@ struct sulimo_hip_seq_batch {
   int n_load_tiles = 0;
   bool load_ready = false;
   sulimo::StepPlan paged_plan, packed_plan;
+  sulimo::StepArray verify_counters;
 };
 
 namespace sulimo {

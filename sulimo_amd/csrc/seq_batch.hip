@@ -115,7 +115,7 @@ int32_t sulimo_hip_seq_batch_create(sulimo_hip_ctx *ctx, size_t head_count, size
 int32_t sulimo_hip_seq_batch_release(sulimo_hip_seq_batch *b) {
   if (!b) return SULIMO_HIP_OK;
   hipError_t e = hipSetDevice(b->device);
-  for (StepArray *a : {&b->seqs, &b->load_tiles, &b->paged_plan.lists, &b->packed_plan.lists}) {
+  for (StepArray *a : {&b->seqs, &b->load_tiles, &b->paged_plan.lists, &b->packed_plan.lists, &b->verify_counters}) {
     // hipFree waits for work that may still use the allocation
     const hipError_t f = a->dev ? hipFree(a->dev) : hipSuccess;
     if (e == hipSuccess) e = f;
