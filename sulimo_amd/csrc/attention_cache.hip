@@ -6,23 +6,28 @@
 // The work is the cache's bytes, 34 per 32 values and read once for all query heads of a KV
 // head and all rows of a tile; 4 d flops per (row, key) are few next to them.
 //
-// A wave takes one KV head and 32 query rows (kCacheRows, rows past the sequence's are
-// computed on and dropped) and runs over key tiles of 32 (head_dim 128) or 64 (64) positions:
-//   - A lane loads 68 bytes, two Q8_0 blocks, as whole dwords (block pairs start at 4-byte
-//     aligned addresses): half a key of 128, or a whole key of 64. The loads of the next tile
-//     are issued before this one is computed, the page-table entries two tiles ahead and
-//     before the loads, so that waiting for an entry does not wait for data behind it.
+// A wave takes one KV head and RT tiles of 16 query rows (rows past the sequence's are computed
+// on and dropped) and runs over key tiles of 32 (head_dim 128) or 64 (64) positions:
+//   - The tile's rows of the head come as 8-byte units, consecutive lanes along a row: lanes that
+//     each took their own key's bytes read at 4.0 to 4.4 TB/s (every load touched 64 lines),
+//     this order at 5.3 to 5.7. They go through the wave's LDS, from where a lane takes blocks
+//     of keys as whole dwords. K of the next tile and V of this one are in flight while the
+//     other is worked on.
 //   - Codes become f16 exactly: byte ^ 0x80 under the exponent of 1024 is 1152 + code; minus
-//     1152, times the block's scale (one f16 rounding, as the ring's window has it).
-//   - S^T = K Q^T by v_mfma_f32_32x32x16_f16 with K from registers as A; the contraction runs
-//     over the head dimensions in whatever order the lanes hold them, and Q^T has the same.
-//     (A 64-wide head: lane l holds key l, and lane halves exchange chunks so that either half
-//     of the wave holds dimensions of the same 32 keys.)
+//     1152, times the block's scale. For K what that rounding drops is kept as a second f16
+//     operand and the weights are split in the same way, for the result's sake: the roundings of
+//     K, V, weights and result would each add 2e-4 of the result, in squares; without the
+//     first and third a result is as near to the 64-bit one as with f16 keys in hand.
+//   - S^T = K Q^T by v_mfma_f32_16x16x32_f16 with K from registers as A: lane (r, g) holds a block
+//     of key r (a 64-wide head: block g mod 2 of key r + 16 (g / 2), and lane halves exchange
+//     chunks). The contraction runs over a block's dimensions in the order in which they lie
+//     in dwords: blocks of odd number start in the middle of one, so theirs is rotated by two
+//     (positions 2 .. 31, 0, 1 hold dimensions 0 .. 29, 30, 31), and Q^T has the same.
 //   - softmax: running max and sum per lane (a lane's scores belong to one row), the max moved
-//     only when a tile exceeds it by 2^8 (P <= 256: exact to f16 precision), sums in f32.
-//   - V goes through the wave's own LDS rows (f16, padded by 32 bytes: neither the writes nor the
-//     reads meet in a bank) and comes back transposed by ds_read_tr16, 4 keys of one dimension
-//     a lane: O^T += V^T P^T with P^T straight from the registers of S^T.
+//     only when a tile exceeds it by 2^8, sums in f32.
+//   - V goes back to LDS as f16 rows (the same order of dimensions, padded so that neither the
+//     writes nor the reads meet in a bank) and comes out transposed by ds_read_tr16, 4 keys of
+//     one dimension a lane: O^T += V^T P^T with P^T straight from the registers of S^T.
 // Waves of a head add up through LDS; pieces of a row tile (several workgroups, few rows over
 // a long cache) leave f32 records, and the workgroup that arrives last joins them in piece
 // order, so the result does not depend on who that is.
@@ -33,7 +38,8 @@
 namespace sulimo {
 namespace {
 
-typedef uint32_t u32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2a4 __attribute__((ext_vector_type(2), aligned(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct CacheAttn {
   SeqView v;
@@ -41,322 +47,432 @@ struct CacheAttn {
   const _Float16 *q;  // [rows][n_head][HD]
   _Float16 *out;
   const uint8_t *k, *vc;  // the cache
-  int n_head, n_head_kv;
+  int n_head, n_head_kv, heads;  // heads: KV heads of a workgroup
   FastDiv page;
   Join join;
 };
 
-// A lane's two blocks of one key: dwords 0 .. 16 from the pair's start.
-struct Raw {
-  uint32_t w[17];
-};
-__device__ __forceinline__ Raw load_raw(const uint8_t *p) {
-  Raw r;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const u32x4a4 v = *reinterpret_cast<const u32x4a4 *>(p + 16 * i);
-#pragma unroll
-    for (int e = 0; e < 4; e++) r.w[4 * i + e] = v[e];
+// A tile of the head's rows on its way to LDS: kUnits 8-byte units, unit 64 j + lane in register
+// j. A row of 136 bytes is 17 units, one of 68 is 8 and a last one that repeats a dword.
+constexpr int kUnits = 9;
+template <int HD>
+__device__ __forceinline__ void unit_of(int j, int lane, int *row, int *dword) {
+  if constexpr (HD == 128) {
+    const int e = min(64 * j + lane, 32 * 17 - 1);
+    *row = e / 17;
+    *dword = 2 * (e - 17 * *row);
+  } else {
+    const int e = 64 * j + lane;
+    *row = e / 9;
+    *dword = min(2 * (e - 9 * *row), 15);
   }
-  r.w[16] = *reinterpret_cast<const uint32_t *>(p + 64);
-  return r;
 }
-// Codes 8c .. 8c + 7 of the 64 as f16(code * scale); codes in the sign-flipped form.
-template <int C>
-__device__ __forceinline__ half8 chunk(const uint32_t (&x)[17], half2v d0, half2v d1) {
+struct Raw {
+  u32x2a4 u[kUnits];
+};
+
+// One Q8_0 block of a lane as it lies in dwords 0 .. 8 from its pair's start (even blocks) or
+// from the dword that ends the one before (odd): codes with their sign bits flipped.
+struct Block {
+  uint32_t x[9], first;  // first: the dword whose high half is position pair 0
+  half2v d;
+};
+// sel: where the scale is in dword 0
+__device__ __forceinline__ Block load_block(const uint32_t *p, bool odd, uint32_t sel) {
+  Block b;
+#pragma unroll
+  for (int i = 0; i < 9; i++) b.x[i] = p[i];
+  b.d = as_h2(__builtin_amdgcn_perm(b.x[0], b.x[0], sel));
+#pragma unroll
+  for (int i = 0; i < 9; i++) b.x[i] ^= 0x80808080u;
+  b.first = odd ? b.x[8] : b.x[0];
+  return b;
+}
+// Positions 8c .. 8c + 7 as f16(code * scale); lo receives what that rounding dropped, exactly.
+template <int C, bool LO>
+__device__ __forceinline__ half8 chunk(const Block &b, half8 *lo = nullptr) {
   const half2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-  const half2v d = C < 4 ? d0 : d1;
   half8 o;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    // halfword of the pair: block 0's codes start at halfword 1, block 1's at 18
-    const int h = C < 4 ? 1 + 4 * C + e : 18 + 4 * (C - 4) + e;
-    const half2v v = (as_h2(__builtin_amdgcn_perm(0x64646464u, x[h >> 1], h & 1 ? 0x04030402u : 0x04010400u)) + off) * d;
+    const int pair = 4 * C + e, h = pair + 1;  // pair j >= 1 is halfword j + 1
+    const uint32_t w = pair ? b.x[h >> 1] : b.first;
+    const half2v c = as_h2(__builtin_amdgcn_perm(0x64646464u, w, !pair || (h & 1) ? 0x04030402u : 0x04010400u)) + off;
+    const half2v v = c * b.d;
     o[2 * e] = v[0];
     o[2 * e + 1] = v[1];
+    if constexpr (LO) {
+      const half2v r = __builtin_elementwise_fma(c, b.d, -v);
+      (*lo)[2 * e] = r[0];
+      (*lo)[2 * e + 1] = r[1];
+    }
   }
   return o;
 }
+template <bool LO>
+__device__ __forceinline__ void chunks(const Block &b, half8 (&hi)[4], half8 (&lo)[4]) {
+  hi[0] = chunk<0, LO>(b, &lo[0]);
+  hi[1] = chunk<1, LO>(b, &lo[1]);
+  hi[2] = chunk<2, LO>(b, &lo[2]);
+  hi[3] = chunk<3, LO>(b, &lo[3]);
+}
 
-template <int HD>
-__global__ __launch_bounds__(512, 2) void cache_attn_kernel(CacheAttn a) {
-  constexpr int KT = HD == 128 ? 32 : 64, NS = KT / 32;  // keys of a tile, S^T tiles
-  constexpr int OT = HD / 32, QS = HD / 16;
-  constexpr int ROW = HD * 2 + 32, WB = KT * ROW;        // LDS bytes of a V row and of a wave
-  static_assert(WB >= 4096, "a wave's LDS also passes one O^T tile");
+// max over the four lanes r, r + 16, r + 32, r + 48
+__device__ __forceinline__ float quad_max(float v) {
+  v = half_swap_max(v);
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+// RT: tiles of 16 rows a wave. WHOLE: tiles end inside no page.
+template <int HD, int RT, bool WHOLE>
+__global__ __launch_bounds__(64 * kCacheWaves, 2) void cache_attn_kernel(CacheAttn a) {
+  constexpr int KT = HD == 128 ? 32 : 64, MT = KT / 16;  // keys of a tile, S^T tiles of 16 keys
+  constexpr int OT = HD / 16;                            // O^T tiles of 16 dimensions
+  constexpr int QS = HD / 32;                            // contraction steps of S^T
+  constexpr int RD = HD == 128 ? 34 : 19;                // dwords of a raw row in LDS: reads of 32 lanes meet in no bank
+  constexpr int ROW = HD == 128 ? 288 : 144;             // LDS bytes of a V row
+  constexpr int OROW = HD + 4;                           // floats of a row of sums in LDS
+  constexpr int WB = KT * ROW > 16 * RT * OROW * 4 ? KT * ROW : 16 * RT * OROW * 4;  // LDS bytes of a wave
+  static_assert(KT * ROW >= KT * RD * 4 + 512, "a wave's LDS also holds raw rows");
   __shared__ __attribute__((aligned(16))) char lds[kCacheWaves][WB];
-  __shared__ float2 lml[kCacheWaves][32];
+  __shared__ float2 lml[kCacheWaves][16 * RT];
   __shared__ int last_one;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, lg = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
   const AttnPiece pc = a.pieces[blockIdx.x];
-  const int heads = a.n_head_kv % 8 == 0 ? 8 : a.n_head_kv % 4 == 0 ? 4 : a.n_head_kv % 2 == 0 ? 2 : 1;
+  const int heads = a.heads;
   const int sub = kCacheWaves / heads;
   const int kvh = blockIdx.y * heads + wave / sub, sw = wave % sub;
   const int G = a.n_head / a.n_head_kv;
   const int off = a.v.off[pc.seq], n = a.v.off[pc.seq + 1] - off, start = a.v.start[pc.seq];
-  const int live = min(kCacheRows, n * G - pc.row0);
-  const int r = pc.row0 + min(l32, live - 1);  // dead rows repeat the last one
-  const int t = r / G, h = kvh * G + r % G;
-  const int P = start + t, Pmin = start + pc.row0 / G, Pmax = start + (pc.row0 + live - 1) / G;
+  const int live = min(16 * RT, n * G - pc.row0);
+  const int Pmin = start + pc.row0 / G, Pmax = start + (pc.row0 + live - 1) / G;
   const int win = a.v.window ? a.v.window : INT_MAX;
   const float c = 1.4426950408889634f / sqrtf((float)HD);
+  const int blk = HD == 128 ? (g >> 1) | (g & 1) << 1 : g & 1;  // the lane's block of a head
+  const bool odd = blk & 1;
+  // dimension pair (of the block's 16) at position pair j
+  const int turn = odd ? 15 : 0;
 
   // Q^T (B operand) in the lanes' order of dimensions
-  half8 qf[QS];
-  {
-    const _Float16 *src = a.q + ((size_t)(off + t) * a.n_head + h) * HD;
+  half8 qf[RT][QS];
+  int P[RT];
 #pragma unroll
-    for (int s = 0; s < QS; s++) qf[s] = *reinterpret_cast<const half8 *>(src + (HD == 128 ? 64 * lg + 8 * s : 16 * s + 8 * lg));
+  for (int x = 0; x < RT; x++) {
+    const int r = pc.row0 + min(16 * x + r16, live - 1);  // dead rows repeat the last one
+    const int t = r / G;
+    P[x] = start + t;
+    const _Float16 *q = a.q + ((size_t)(off + t) * a.n_head + kvh * G + r % G) * HD + 32 * blk;
+#pragma unroll
+    for (int s = 0; s < QS; s++) {
+      const int ch = HD == 128 ? s : 2 * s + (g >> 1);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const half2v y = *reinterpret_cast<const half2v *>(q + 2 * ((4 * ch + e + turn) & 15));
+        qf[x][s][2 * e] = y[0];
+        qf[x][s][2 * e + 1] = y[1];
+      }
+    }
   }
 
   const int32_t *table = a.v.pages + a.v.page_off[pc.seq];
   const uint32_t row_bytes = (uint32_t)a.n_head_kv * (HD / 32) * 34;
-  const uint32_t col = (uint32_t)kvh * (HD / 32) * 34 + (HD == 128 ? 68 * lg : 0);
-  const int klane = HD == 128 ? l32 : lane;  // the tile's key of this lane
-  auto page_of = [&](int tile, uint32_t *in_page) __attribute__((always_inline)) {
-    const uint32_t p = (uint32_t)min(tile * KT + klane, Pmax);  // tiles end inside a page or past the last position
-    const uint32_t pg = (uint32_t)((uint64_t)p * a.page.magic >> a.page.shift);
-    *in_page = p - pg * a.page.d;
-    return table[pg];
+  const uint32_t col = (uint32_t)kvh * (HD / 32) * 34;
+  // Where a tile lies: WHOLE, its first byte; else the cache row of each lane's key. Keys past
+  // the last position stand for it.
+  struct Place {
+    size_t at;
+    uint32_t slot;
   };
-
-  floatx16 o[OT];
+  auto place = [&](int tile) __attribute__((always_inline)) {
+    Place w{};
+    if constexpr (WHOLE) {
+      const uint32_t p = (uint32_t)min(tile * KT, Pmax), pg = (uint32_t)((uint64_t)p * a.page.magic >> a.page.shift);
+      const uint32_t slot = __builtin_amdgcn_readfirstlane((uint32_t)table[pg] * a.page.d + (p - pg * a.page.d));
+      w.at = (size_t)slot * row_bytes + col;
+    } else {
+      const uint32_t p = (uint32_t)min(tile * KT + (lane & (KT - 1)), Pmax);
+      const uint32_t pg = (uint32_t)((uint64_t)p * a.page.magic >> a.page.shift);
+      w.slot = (uint32_t)table[pg] * a.page.d + (p - pg * a.page.d);
+    }
+    return w;
+  };
+  auto fetch = [&](const uint8_t *cache, const Place &w, Raw &x) __attribute__((always_inline)) {
+    int lane = tid & 63;
+    if constexpr (!WHOLE || RT > 1) asm volatile("" : "+v"(lane));  // the units' rows and offsets are not worth 18 registers
 #pragma unroll
-  for (int i = 0; i < OT; i++) o[i] = floatx16{};
-  float mrun = -INFINITY, lrun = 0.0f;
-  char *vrow = lds[wave] + klane * ROW + (HD == 128 ? 128 * lg : 0);
-  const char *vread = lds[wave] + (4 * lg + ((lane & 15) >> 2)) * ROW + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    for (int j = 0; j < kUnits; j++) {
+      int row, dw;
+      unit_of<HD>(j, lane, &row, &dw);
+      if constexpr (WHOLE) {
+        x.u[j] = *reinterpret_cast<const u32x2a4 *>((cache + w.at) + ((uint32_t)row * row_bytes + 4 * dw));
+      } else {
+        const size_t o = (size_t)(uint32_t)__shfl((int)w.slot, row, 64) * row_bytes + (col + 4 * dw);
+        x.u[j] = *reinterpret_cast<const u32x2a4 *>(cache + o);
+      }
+    }
+  };
+  char *mine = lds[wave];
+  auto stage = [&](const Raw &x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kUnits; j++) {
+      if constexpr (HD == 128) {  // rows back to back: unit e at 8 e (the lanes past the last unit write behind it)
+        reinterpret_cast<u32x2a4 *>(mine)[64 * j + lane] = x.u[j];
+      } else {
+        int row, dw;
+        unit_of<HD>(j, lane, &row, &dw);
+        *reinterpret_cast<u32x2a4 *>(reinterpret_cast<uint32_t *>(mine) + row * RD + dw) = x.u[j];
+      }
+    }
+  };
+  // the lane's two keys of a tile: key0, and key0 + step
+  const int key0 = HD == 128 ? r16 : 16 * (g >> 1) + r16;
+  constexpr int kStep = HD == 128 ? 16 : 32;
+  const uint32_t *blk0 = reinterpret_cast<const uint32_t *>(mine) + key0 * RD + 17 * (blk >> 1) + 8 * (blk & 1);
+  const uint32_t scale_sel = odd ? 0x03020302u : 0x01000100u;
+  char *vrow = mine + key0 * ROW + 64 * blk;
+  const char *vread = mine + (4 * g + (r16 >> 2)) * ROW + 8 * (r16 & 3);
 
-  auto compute = [&](const Raw &kr, const Raw &vr, int tile) __attribute__((always_inline)) {
+  floatx4 o[RT][OT];
+  float mrun[RT], lrun[RT];
+#pragma unroll
+  for (int x = 0; x < RT; x++) {
+#pragma unroll
+    for (int i = 0; i < OT; i++) o[x][i] = floatx4{};
+    mrun[x] = -INFINITY;
+    lrun[x] = 0.0f;
+  }
+
+  half8 pf[RT][KT / 32], pl[RT][KT / 32];  // the tile's weights, and what their rounding dropped
+  // S^T of the K rows in LDS, and the weights
+  auto scores = [&](int tile) __attribute__((always_inline)) {
     const int k0 = tile * KT;
-    const bool masked = k0 + KT - 1 > Pmin || k0 <= Pmax - win;
-    // S^T
-    floatx16 st[NS];
-    {
-      uint32_t x[17];
+    floatx4 st[RT][MT];
 #pragma unroll
-      for (int i = 0; i < 17; i++) x[i] = kr.w[i] ^ 0x80808080u;
-      const half2v d0 = as_h2(__builtin_amdgcn_perm(kr.w[0], kr.w[0], 0x01000100u));
-      const half2v d1 = as_h2(__builtin_amdgcn_perm(kr.w[8], kr.w[8], 0x03020302u));
-      half8 f[8] = {chunk<0>(x, d0, d1), chunk<1>(x, d0, d1), chunk<2>(x, d0, d1), chunk<3>(x, d0, d1),
-                    chunk<4>(x, d0, d1), chunk<5>(x, d0, d1), chunk<6>(x, d0, d1), chunk<7>(x, d0, d1)};
+    for (int x = 0; x < RT; x++)
 #pragma unroll
-      for (int i = 0; i < NS; i++) st[i] = floatx16{};
+      for (int m = 0; m < MT; m++) st[x][m] = floatx4{};
+    auto product = [&](half8 k, int s, int m) __attribute__((always_inline)) {
+#pragma unroll
+      for (int x = 0; x < RT; x++) st[x][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[x][s], st[x][m], 0, 0, 0);
+    };
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      half8 hi[4], lo[4];
+      chunks<true>(load_block(blk0 + u * kStep * RD, odd, scale_sel), hi, lo);
       if constexpr (HD == 128) {
 #pragma unroll
-        for (int s = 0; s < QS; s++) st[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[s], qf[s], st[0], 0, 0, 0);
-      } else {
-#pragma unroll
         for (int s = 0; s < QS; s++) {
-          typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-          u32x4 u = __builtin_bit_cast(u32x4, f[2 * s]), v = __builtin_bit_cast(u32x4, f[2 * s + 1]);
+          product(hi[s], s, u);
+          product(lo[s], s, u);
+        }
+      } else {
+        auto both = [&](half8 p, half8 q, int s) __attribute__((always_inline)) {
+          u32x4 y = __builtin_bit_cast(u32x4, p), z = __builtin_bit_cast(u32x4, q);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const auto w = __builtin_amdgcn_permlane32_swap(u[e], v[e], false, false);
-            u[e] = w[0];
-            v[e] = w[1];
+            const auto w = __builtin_amdgcn_permlane32_swap(y[e], z[e], false, false);
+            y[e] = w[0];
+            z[e] = w[1];
           }
-          st[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, u), qf[s], st[0], 0, 0, 0);
-          st[NS - 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, v), qf[s], st[NS - 1], 0, 0, 0);
+          product(__builtin_bit_cast(half8, y), s, 2 * u);
+          product(__builtin_bit_cast(half8, z), s, 2 * u + 1);
+        };
+#pragma unroll
+        for (int s = 0; s < QS; s++) {
+          both(hi[2 * s], hi[2 * s + 1], s);
+          both(lo[2 * s], lo[2 * s + 1], s);
         }
       }
     }
-    // V rows to LDS. A block whose scale is not finite makes every row that sees its key NaN;
-    // in tiles where some rows do not, it is set to zero and the others are marked.
-    half2v d0 = as_h2(__builtin_amdgcn_perm(vr.w[0], vr.w[0], 0x01000100u));
-    half2v d1 = as_h2(__builtin_amdgcn_perm(vr.w[8], vr.w[8], 0x03020302u));
+    if (k0 + KT - 1 > Pmin || k0 <= Pmax - win) {
+#pragma unroll
+      for (int x = 0; x < RT; x++)
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int p = k0 + 16 * m + 4 * g + e;
+            st[x][m][e] = (p > P[x] || p <= P[x] - win) ? -INFINITY : st[x][m][e];
+          }
+    }
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+      float mt = -INFINITY;
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) mt = fmaxf(mt, st[x][m][e]);
+      mt = quad_max(mt) * c;
+      const bool grow = mt > mrun[x] + kLazy;
+      const float alpha = grow && mrun[x] != -INFINITY ? __builtin_amdgcn_exp2f(mrun[x] - mt) : 1.0f;
+      if (grow) mrun[x] = mt;
+      const float ms = mrun[x] == -INFINITY ? 0.0f : mrun[x];  // no key seen yet: exp2(-inf) = 0
+      float sum = 0.0f;
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][m][e], c, -ms));
+          const _Float16 h = (_Float16)w;
+          pf[x][m >> 1][4 * (m & 1) + e] = h;
+          pl[x][m >> 1][4 * (m & 1) + e] = (_Float16)(w - (float)h);
+          sum += w;
+        }
+      lrun[x] = lrun[x] * alpha + sum;
+      if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+        for (int i = 0; i < OT; i++) o[x][i] *= alpha;
+      }
+    }
+  };
+  // O^T += V^T P^T of the raw V rows in LDS, which become f16 rows there. A block whose scale is
+  // not finite makes every row that sees its key NaN; in tiles that some rows do not see as a
+  // whole, it is set to zero and the others are marked.
+  auto values = [&](int tile) __attribute__((always_inline)) {
+    const int k0 = tile * KT;
+    const bool masked = k0 + KT - 1 > Pmin || k0 <= Pmax - win;
+    Block b0 = load_block(blk0, odd, scale_sel), b1 = load_block(blk0 + kStep * RD, odd, scale_sel);
     uint64_t bad0 = 0, bad1 = 0;
     if (masked) {
-      const bool b0 = (vr.w[0] & 0x7c00u) == 0x7c00u, b1 = (vr.w[8] & 0x7c000000u) == 0x7c000000u;
-      bad0 = __ballot(b0);
-      bad1 = __ballot(b1);
-      if (b0) d0 = half2v{0, 0};
-      if (b1) d1 = half2v{0, 0};
+      auto off_scale = [](half2v d) { return (__builtin_bit_cast(uint32_t, d) & 0x7c00u) == 0x7c00u; };
+      bad0 = __ballot(off_scale(b0.d));
+      bad1 = __ballot(off_scale(b1.d));
+      if (off_scale(b0.d)) b0.d = half2v{0, 0};
+      if (off_scale(b1.d)) b1.d = half2v{0, 0};
     }
-    {
-      uint32_t x[17];
+    half8 y[4], z[4], none[4];
+    chunks<false>(b0, y, none);
+    chunks<false>(b1, z, none);
 #pragma unroll
-      for (int i = 0; i < 17; i++) x[i] = vr.w[i] ^ 0x80808080u;
-      half8 *dst = reinterpret_cast<half8 *>(vrow);
-      dst[0] = chunk<0>(x, d0, d1);
-      dst[1] = chunk<1>(x, d0, d1);
-      dst[2] = chunk<2>(x, d0, d1);
-      dst[3] = chunk<3>(x, d0, d1);
-      dst[4] = chunk<4>(x, d0, d1);
-      dst[5] = chunk<5>(x, d0, d1);
-      dst[6] = chunk<6>(x, d0, d1);
-      dst[7] = chunk<7>(x, d0, d1);
+    for (int i = 0; i < 4; i++) {
+      reinterpret_cast<half8 *>(vrow)[i] = y[i];
+      reinterpret_cast<half8 *>(vrow + kStep * ROW)[i] = z[i];
     }
-    if (masked) {
+    // registers 4 m .. of S^T are keys 16 m + 4 g + {0-3}: a step takes m = 2 kk and 2 kk + 1
 #pragma unroll
-      for (int i = 0; i < NS; i++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const int p = k0 + 32 * i + 8 * (e >> 2) + 4 * lg + (e & 3);
-          st[i][e] = (p > P || p <= P - win) ? -INFINITY : st[i][e];
-        }
-    }
-    // softmax
-    float mt = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NS; i++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) mt = fmaxf(mt, st[i][e]);
-    mt = half_swap_max(mt) * c;
-    const bool grow = mt > mrun + kLazy;
-    const float alpha = grow && mrun != -INFINITY ? __builtin_amdgcn_exp2f(mrun - mt) : 1.0f;
-    if (grow) mrun = mt;
-    const float ms = mrun == -INFINITY ? 0.0f : mrun;  // no key seen yet: exp2(-inf) = 0
-    half8 pf[2 * NS];
-    const half2v one = {(_Float16)1.0f, (_Float16)1.0f};
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NS; i++)
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const half2v w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[i][e], c, -ms)),
-                          (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[i][e + 1], c, -ms))};
-        sum = __builtin_amdgcn_fdot2(w, one, sum, false);  // the f16 weights the products use
-        pf[2 * i + (e >> 3)][e & 7] = w[0];
-        pf[2 * i + (e >> 3)][(e & 7) + 1] = w[1];
-      }
-    lrun = lrun * alpha + sum;
-    if (__ballot(alpha != 1.0f)) {
-#pragma unroll
-      for (int i = 0; i < OT; i++) o[i] *= alpha;
-    }
-    // O^T += V^T P^T, 16 keys a step: registers 8 kk .. of S^T are keys 16 kk + {0-3, 8-11} + 4 lg
-#pragma unroll
-    for (int kk = 0; kk < KT / 16; kk++)
+    for (int kk = 0; kk < KT / 32; kk++)
 #pragma unroll
       for (int i = 0; i < OT; i++) {
-        const char *src = vread + 16 * kk * ROW + 64 * i;
-        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read_tr(src, src + 8 * ROW), pf[kk], o[i], 0, 0, 0);
+        const char *src = vread + 32 * kk * ROW + 32 * i;
+        const half8 vf = read_tr(src, src + 16 * ROW);
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+          o[x][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[x][kk], o[x][i], 0, 0, 0);
+          o[x][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[x][kk], o[x][i], 0, 0, 0);
+        }
       }
     if (masked && (bad0 | bad1)) {
-      // keys of this tile that the row sees
-      uint64_t sees = ~0ull;
-      const int up = P - k0, dn = P - win < k0 ? 0 : P - win - k0 + 1;  // keys dn .. up
-      sees = up < 0 ? 0 : up >= 63 ? sees : (2ull << up) - 1;
-      sees = dn >= 64 ? 0 : sees & (~0ull << dn);
 #pragma unroll
-      for (int i = 0; i < OT; i++) {  // O^T tile i is block i of the head
-        uint64_t b = (i & 1) ? bad1 : bad0;
-        if constexpr (HD == 128) b = (uint32_t)(b >> (32 * (i >> 1)));
-        const float x = (b & sees) ? __builtin_nanf("") : 0.0f;
+      for (int x = 0; x < RT; x++) {
+        // keys of this tile that the row sees
+        uint64_t sees = ~0ull;
+        const int up = P[x] - k0, dn = P[x] - win < k0 ? 0 : P[x] - win - k0 + 1;  // keys dn .. up
+        sees = up < 0 ? 0 : up >= 63 ? sees : (2ull << up) - 1;
+        sees = dn >= 64 ? 0 : sees & (~0ull << dn);
 #pragma unroll
-        for (int e = 0; e < 16; e++) o[i][e] += x;
+        for (int i = 0; i < OT; i++) {  // block i / 2 of the head
+          auto keys = [&](uint64_t bad, int at) { return (bad >> (16 * at)) & 0xffffull; };
+          uint64_t b;
+          constexpr int at[4] = {0, 2, 1, 3};  // the lanes of a block
+          if constexpr (HD == 128) b = keys(bad0, at[i >> 1]) | keys(bad1, at[i >> 1]) << 16;
+          else b = keys(bad0, i >> 1) | keys(bad0, 2 + (i >> 1)) << 16 | keys(bad1, i >> 1) << 32 | keys(bad1, 2 + (i >> 1)) << 48;
+          const float nan = (b & sees) ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[x][i][e] += nan;
+        }
       }
     }
   };
 
-  // key tiles tile0 + sw, + sub, ... of this wave
-  {
-    int tile = pc.tile0 + sw;
-    const uint8_t *kb = a.k + col, *vb = a.vc + col;
-    uint32_t in0, in1;
-    int32_t pg0 = 0, pg1 = 0;
-    Raw k0, v0, k1, v1;
-    auto fetch = [&](Raw &k, Raw &v, int32_t pg, uint32_t in) __attribute__((always_inline)) {
-      const size_t at = ((size_t)(uint32_t)pg * a.page.d + in) * row_bytes;
-      k = load_raw(kb + at);
-      v = load_raw(vb + at);
-    };
-    if (tile < pc.tile1) {
-      pg0 = page_of(tile, &in0);
-      pg1 = page_of(tile + sub, &in1);
-      fetch(k0, v0, pg0, in0);
-      for (;;) {
-        // two tiles a turn, so that no register moves between the buffers
-        pg0 = page_of(tile + 2 * sub, &in0);
-        if (tile + sub < pc.tile1) fetch(k1, v1, pg1, in1);
-        compute(k0, v0, tile);
-        tile += sub;
-        if (tile >= pc.tile1) break;
-        pg1 = page_of(tile + 2 * sub, &in1);
-        if (tile + sub < pc.tile1) fetch(k0, v0, pg0, in0);
-        compute(k1, v1, tile);
-        tile += sub;
-        if (tile >= pc.tile1) break;
-      }
+  // key tiles tile0 + sw, + sub, ... of this wave; the loads of a tile are issued as soon as the
+  // registers of the one before are in LDS
+  // (two row tiles leave registers for one of the two, so half a tile ahead)
+  if (pc.tile0 + sw < pc.tile1) {
+    Raw k, v;
+    Place at = place(pc.tile0 + sw), next = place(pc.tile0 + sw + sub);
+    fetch(a.k, at, k);
+    if constexpr (RT == 1) fetch(a.vc, at, v);
+    for (int tile = pc.tile0 + sw; tile < pc.tile1; tile += sub) {
+      const bool more = tile + sub < pc.tile1;
+      stage(k);
+      if constexpr (RT > 1) fetch(a.vc, at, v);
+      else if (more) fetch(a.k, next, k);
+      scores(tile);
+      stage(v);
+      if (more) fetch(RT > 1 ? a.k : a.vc, next, RT > 1 ? k : v);
+      at = next;
+      next = place(tile + 2 * sub);
+      values(tile);
     }
   }
 
-  // ---- the waves of a head: joint max and sum, then O^T tile by tile ----
-  lrun += __shfl_xor(lrun, 32, 64);  // lane halves hold different keys
+  // ---- the waves of a head: sums of the live rows to LDS, [row][dimension] ----
+  float *sums = reinterpret_cast<float *>(mine);
+#pragma unroll
+  for (int x = 0; x < RT; x++) {
+    lrun[x] += __shfl_xor(lrun[x], 16, 64);  // lanes of a row hold different keys
+    lrun[x] += __shfl_xor(lrun[x], 32, 64);
+    if (16 * x + r16 >= live) continue;
+    if (g == 0) lml[wave][16 * x + r16] = float2{mrun[x], lrun[x]};
+#pragma unroll
+    for (int i = 0; i < OT; i++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        // position pairs 2 g and 2 g + 1 (+ 8 for odd tiles) of block i / 2
+        const int pair = (8 * (i & 1) + 2 * g + e + (i & 2 ? 15 : 0)) & 15;
+        *reinterpret_cast<float2 *>(sums + (16 * x + r16) * OROW + 32 * (i >> 1) + 2 * pair) = float2{o[x][i][2 * e], o[x][i][2 * e + 1]};
+      }
+  }
+  __syncthreads();
+  // four dimensions of a row a thread
   const int w0 = wave - sw;
-  float M = mrun;
-  if (sub > 1) {
-    if (lg == 0) lml[wave][l32] = float2{mrun, lrun};
-    __syncthreads();
-    float L = 0.0f;
-    for (int j = 0; j < sub; j++) M = fmaxf(M, lml[w0 + j][l32].x);
-    const float Ms = M == -INFINITY ? 0.0f : M;
-    for (int j = 0; j < sub; j++) L += lml[w0 + j][l32].y * __builtin_amdgcn_exp2f(lml[w0 + j][l32].x - Ms);
-    const float mine = __builtin_amdgcn_exp2f(mrun - Ms);
-    lrun = L;
-    // O^T tile i is added up by wave i mod sub of the head, into its o[i]
-#pragma unroll
-    for (int i = 0; i < OT; i++) {
-      float4 *dst = reinterpret_cast<float4 *>(lds[wave]) + lane;
-#pragma unroll
-      for (int g = 0; g < 4; g++)
-        dst[64 * g] = float4{o[i][4 * g] * mine, o[i][4 * g + 1] * mine, o[i][4 * g + 2] * mine, o[i][4 * g + 3] * mine};
-      __syncthreads();
-      if (i % sub == sw) {
-        floatx16 acc{};
-        for (int j = 0; j < sub; j++) {
-          const float4 *src = reinterpret_cast<const float4 *>(lds[w0 + j]) + lane;
-#pragma unroll
-          for (int g = 0; g < 4; g++) {
-            const float4 x = src[64 * g];
-            acc[4 * g] += x.x;
-            acc[4 * g + 1] += x.y;
-            acc[4 * g + 2] += x.z;
-            acc[4 * g + 3] += x.w;
-          }
-        }
-        o[i] = acc;
-      }
-      __syncthreads();
+  for (int job = 64 * sw + lane; job < live * (HD / 4); job += 64 * sub) {
+    const int row = job / (HD / 4), d = 4 * (job % (HD / 4));
+    float m = -INFINITY, l = 0.0f;
+    for (int j = 0; j < sub; j++) m = fmaxf(m, lml[w0 + j][row].x);
+    const float ms = m == -INFINITY ? 0.0f : m;
+    floatx4 acc{};
+    for (int j = 0; j < sub; j++) {
+      const float2 ml = lml[w0 + j][row];
+      const float f = __builtin_amdgcn_exp2f(ml.x - ms);
+      l += ml.y * f;
+      acc += *reinterpret_cast<const floatx4 *>(reinterpret_cast<const float *>(lds[w0 + j]) + row * OROW + d) * f;
+    }
+    if (pc.n_pieces == 1) {
+      const int r = pc.row0 + row;
+      const float inv = 1.0f / l;
+      *reinterpret_cast<half4 *>(a.out + ((size_t)(off + r / G) * a.n_head + kvh * G + r % G) * HD + d) =
+          half4{(_Float16)(acc[0] * inv), (_Float16)(acc[1] * inv), (_Float16)(acc[2] * inv), (_Float16)(acc[3] * inv)};
+    } else {
+      const size_t rr = (size_t)pc.rec + ((size_t)pc.piece * a.n_head_kv + kvh) * live + row;
+      st_dev4(a.join.o + rr * HD + d, acc);
+      if (d == 0) st_dev(a.join.ml + rr, float2{m, l});
     }
   }
+  if (pc.n_pieces > 1 && arrived_last(a.join, pc, blockIdx.y, &last_one))
+    join_pieces<HD, 64 * kCacheWaves>(a.join, pc, blockIdx.y * heads, heads, live, a.n_head, a.n_head_kv,
+                                      a.out + (size_t)off * a.n_head * HD);
+}
 
-  if (pc.n_pieces == 1) {
-    if (l32 >= live) return;
-    const float inv = 1.0f / lrun;
-    _Float16 *dst = a.out + ((size_t)(off + t) * a.n_head + h) * HD + 4 * lg;
-#pragma unroll
-    for (int i = 0; i < OT; i++)
-      if (i % sub == sw) {
-#pragma unroll
-        for (int g = 0; g < 4; g++)
-          *reinterpret_cast<half4 *>(dst + 32 * i + 8 * g) =
-              half4{(_Float16)(o[i][4 * g] * inv), (_Float16)(o[i][4 * g + 1] * inv), (_Float16)(o[i][4 * g + 2] * inv),
-                    (_Float16)(o[i][4 * g + 3] * inv)};
-      }
-    return;
-  }
-
-  if (l32 < live) {
-    const size_t rr = (size_t)pc.rec + ((size_t)pc.piece * a.n_head_kv + kvh) * live + l32;
-    if (sw == 0 && lg == 0) st_dev(a.join.ml + rr, float2{M, lrun});
-#pragma unroll
-    for (int i = 0; i < OT; i++)
-      if (i % sub == sw) record_tile<HD>(a.join, rr, i, lg, o[i]);
-  }
-  if (!arrived_last(a.join, pc, blockIdx.y, &last_one)) return;
-  join_pieces<HD, 512>(a.join, pc, blockIdx.y * heads, heads, live, a.n_head, a.n_head_kv, a.out + (size_t)off * a.n_head * HD);
+template <int HD, int RT>
+void launch(const CacheAttn &a, dim3 grid, hipStream_t s) {
+  if (a.page.d % (HD == 128 ? 32 : 64) == 0) hipLaunchKernelGGL((cache_attn_kernel<HD, RT, true>), grid, dim3(64 * kCacheWaves), 0, s, a);
+  else hipLaunchKernelGGL((cache_attn_kernel<HD, RT, false>), grid, dim3(64 * kCacheWaves), 0, s, a);
 }
 
 }  // namespace
 
-int32_t launch_cache_attention(const StepAttnArgs &c, const uint8_t *k_cache, const uint8_t *v_cache, hipStream_t s) {
-  CacheAttn a{c.v, c.pieces, c.q, c.out, k_cache, v_cache, c.n_head, c.n_head_kv, fast_div((uint32_t)c.v.page_size),
-              c.join};
-  const dim3 grid(c.n_pieces, c.n_head_kv / cache_heads(c.n_head_kv));
-  if (c.head_dim == 64) hipLaunchKernelGGL((cache_attn_kernel<64>), grid, dim3(512), 0, s, a);
-  else hipLaunchKernelGGL((cache_attn_kernel<128>), grid, dim3(512), 0, s, a);
+int32_t launch_cache_attention(const StepAttnArgs &c, int row_tiles, const uint8_t *k_cache, const uint8_t *v_cache, hipStream_t s) {
+  const CacheAttn a{c.v, c.pieces, c.q, c.out, k_cache, v_cache, c.n_head, c.n_head_kv, c.heads,
+                    fast_div((uint32_t)c.v.page_size), c.join};
+  const dim3 grid(c.n_pieces, c.n_head_kv / c.heads);
+  if (c.head_dim == 64 && row_tiles == 1) launch<64, 1>(a, grid, s);
+  else if (c.head_dim == 64) launch<64, 2>(a, grid, s);
+  else if (row_tiles == 1) launch<128, 1>(a, grid, s);
+  else launch<128, 2>(a, grid, s);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? SULIMO_HIP_OK : hip_fail(e, "cache_attn_kernel launch");
 }

@@ -57,9 +57,9 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
   constexpr int NI = kRowKeys / RPI / 4;    // DMA instructions per wave and tile
   __shared__ __attribute__((aligned(16))) char ka[TILE], va[TILE], kb[TILE], vb[TILE];
   __shared__ int shared_flag;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, lg = lane >> 5;
   const int n_head_kv = a.s.n_head_kv, n_head = a.s.n_head, G = n_head / n_head_kv;
   const int kvh = blockIdx.x % n_head_kv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, lg = lane >> 5;
   const AttnPiece pc = a.s.pieces[blockIdx.x / n_head_kv];
   const SeqKv kv = a.kv[pc.seq];
   const int off = a.s.v.off[pc.seq], total = (a.s.v.off[pc.seq + 1] - off) * G, start = a.s.v.start[pc.seq];
@@ -336,27 +336,32 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
   }
 
   lrun += __shfl_xor(lrun, 32, 64);  // lane halves hold different keys
+  const bool mine = wave_live && l32 < wlive;
   if (pc.n_pieces == 1) {
-    if (!wave_live || l32 >= wlive) return;
-    const float inv = 1.0f / lrun;
-    _Float16 *dst = a.s.out + ((size_t)(off + t) * n_head + h) * HD + 4 * lg;
+    if (mine) {
+      const float inv = 1.0f / lrun;
+      _Float16 *dst = a.s.out + ((size_t)(off + t) * n_head + h) * HD + 4 * lg;
 #pragma unroll
-    for (int i = 0; i < OT; i++)
+      for (int i = 0; i < OT; i++)
 #pragma unroll
-      for (int g = 0; g < 4; g++)
-        *reinterpret_cast<half4 *>(dst + 32 * i + 8 * g) =
-            half4{(_Float16)(o[i][4 * g] * inv), (_Float16)(o[i][4 * g + 1] * inv), (_Float16)(o[i][4 * g + 2] * inv),
-                  (_Float16)(o[i][4 * g + 3] * inv)};
-    return;
+        for (int g = 0; g < 4; g++)
+          *reinterpret_cast<half4 *>(dst + 32 * i + 8 * g) =
+              half4{(_Float16)(o[i][4 * g] * inv), (_Float16)(o[i][4 * g + 1] * inv), (_Float16)(o[i][4 * g + 2] * inv),
+                    (_Float16)(o[i][4 * g + 3] * inv)};
+    }
+  } else {
+    if (mine) {
+      const size_t rr = (size_t)pc.rec + ((size_t)pc.piece * n_head_kv + kvh) * live + rl;
+      if (lg == 0) st_dev(a.s.join.ml + rr, float2{mrun, lrun});
+#pragma unroll
+      for (int i = 0; i < OT; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+          st_dev4(a.s.join.o + rr * HD + 32 * i + 8 * g + 4 * lg, floatx4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]});
+    }
+    if (arrived_last(a.s.join, pc, kvh, &shared_flag))
+      join_pieces<HD, 256>(a.s.join, pc, kvh, 1, live, n_head, n_head_kv, a.s.out + (size_t)off * n_head * HD);
   }
-  if (wave_live && l32 < wlive) {
-    const size_t rr = (size_t)pc.rec + ((size_t)pc.piece * n_head_kv + kvh) * live + rl;
-    if (lg == 0) st_dev(a.s.join.ml + rr, float2{mrun, lrun});
-#pragma unroll
-    for (int i = 0; i < OT; i++) record_tile<HD>(a.s.join, rr, i, lg, o[i]);
-  }
-  if (!arrived_last(a.s.join, pc, kvh, &shared_flag)) return;
-  join_pieces<HD, 256>(a.s.join, pc, kvh, 1, live, n_head, n_head_kv, a.s.out + (size_t)off * n_head * HD);
 }
 
 }  // namespace

@@ -25,17 +25,18 @@ int32_t plan(sulimo_hip_seq_batch *b, bool packed) {
   StepPlan &p = packed ? b->packed_plan : b->paged_plan;
   if (p.ready) return SULIMO_HIP_OK;
   const int cus = device_cu_count(), G = b->g.n_head / b->g.n_head_kv;
-  std::vector<int> few, many;
+  std::vector<int> which[3];
   for (int s = 0; s < b->q.n_seqs; s++) {
-    if (b->q.n_new[s] == 0) continue;
-    (!packed && (long)b->q.n_new[s] * G <= kDirectRows ? few : many).push_back(s);
+    const long rows = (long)b->q.n_new[s] * G;
+    if (rows) which[packed || rows > kDirectRows ? 2 : rows > 16 ? 1 : 0].push_back(s);
   }
-  const AttnPlan c = plan_attention_pieces(b->g, b->q, few, cache_split(b->g, cus));
-  const AttnPlan r = plan_attention_pieces(b->g, b->q, many, row_split(cus));
+  const AttnPlan a[3] = {plan_cache_attention(b->g, b->q, which[0], 1, cus),
+                         plan_cache_attention(b->g, b->q, which[1], 2, cus),
+                         plan_attention_pieces(b->g, b->q, which[2], row_split(cus))};
   std::vector<SeqKv> kv(b->q.n_seqs, SeqKv{0, 0, 0});
   std::vector<LoadTile> tiles;
   long rows = 0;
-  for (int s : many) {
+  for (int s : which[2]) {
     const int end = b->q.start[s] + b->q.n_new[s];
     const int lo = first_seen(b->g, b->q.start[s]) / kRowKeys * kRowKeys;
     kv[s] = packed ? SeqKv{b->q.off[s], 0, end} : SeqKv{(int32_t)rows, lo, end - lo};
@@ -48,27 +49,27 @@ int32_t plan(sulimo_hip_seq_batch *b, bool packed) {
       rows += end - lo;
     }
   }
-  // one array: pieces, pieces, where the keys are, load tiles, counters (zero)
-  p.n_cache = (int)c.pieces.size();
-  p.n_rows = (int)r.pieces.size();
+  // one array: the pieces of each list, where the keys are, load tiles, counters (zero)
+  std::vector<char> blob;
+  auto put = [&](const void *src, size_t n) {
+    const size_t at = blob.size();
+    blob.resize(at + align_up(n), 0);
+    if (src && n) memcpy(blob.data() + at, src, n);
+    return at;
+  };
+  p.rec_rows = 0;
+  for (int i = 0; i < 3; i++) {
+    p.list[i].n = (int)a[i].pieces.size();
+    p.list[i].at = put(a[i].pieces.data(), a[i].pieces.size() * sizeof(AttnPiece));
+    p.list[i].counters = put(nullptr, (size_t)a[i].counters * 4);
+    p.list[i].rec = p.rec_rows;
+    p.list[i].heads = a[i].heads;
+    p.rec_rows += a[i].rec_rows;
+  }
+  p.at_kv = put(kv.data(), kv.size() * sizeof(SeqKv));
+  p.at_tiles = put(tiles.data(), tiles.size() * sizeof(LoadTile));
   p.n_tiles = (int)tiles.size();
   p.read_rows = rows;
-  p.cache_rec = c.rec_rows;
-  p.rec_rows = c.rec_rows + r.rec_rows;
-  p.at_rows = align_up(c.pieces.size() * sizeof(AttnPiece));
-  p.at_kv = p.at_rows + align_up(r.pieces.size() * sizeof(AttnPiece));
-  p.at_tiles = p.at_kv + align_up(kv.size() * sizeof(SeqKv));
-  p.at_cache_counters = p.at_tiles + align_up(tiles.size() * sizeof(LoadTile));
-  p.at_row_counters = p.at_cache_counters + align_up((size_t)c.counters * 4);
-  std::vector<char> blob(p.at_row_counters + align_up((size_t)r.counters * 4), 0);
-  auto put = [&](size_t at, const void *src, size_t n) {
-    if (n) memcpy(blob.data() + at, src, n);
-  };
-  put(0, c.pieces.data(), c.pieces.size() * sizeof(AttnPiece));
-  put(p.at_rows, r.pieces.data(), r.pieces.size() * sizeof(AttnPiece));
-  put(p.at_kv, kv.data(), kv.size() * sizeof(SeqKv));
-  put(p.at_tiles, tiles.data(), tiles.size() * sizeof(LoadTile));
-  if (blob.empty()) blob.resize(256, 0);
   STEP_TRY(step_array(b, &p.lists, blob.size()));
   SULIMO_HIP_TRY(hipMemcpyAsync(p.lists.dev, blob.data(), blob.size(), hipMemcpyHostToDevice, b->ctx->stream));
   p.ready = true;
@@ -83,32 +84,25 @@ int32_t attend(sulimo_hip_seq_batch *b, StepPlan &p, const uint16_t *q, const ui
   const size_t kv_bytes = align_up((size_t)p.read_rows * width * 2);
   STEP_TRY(ensure_workspace(ctx, o_bytes + ml_bytes + 2 * kv_bytes));
   char *ws = reinterpret_cast<char *>(ctx->ws), *lists = reinterpret_cast<char *>(p.lists.dev);
-  float *rec_o = reinterpret_cast<float *>(ws);
-  float2 *rec_ml = reinterpret_cast<float2 *>(ws + o_bytes);
-  const StepAttnArgs base{seq_view(b), nullptr, 0, reinterpret_cast<const _Float16 *>(q),
-                          reinterpret_cast<_Float16 *>(out), b->g.n_head, b->g.n_head_kv, b->g.head_dim, Join{}};
-  if (p.n_cache) {
-    StepAttnArgs c = base;
-    c.pieces = reinterpret_cast<const AttnPiece *>(lists);
-    c.n_pieces = p.n_cache;
-    c.join = Join{rec_o, rec_ml, reinterpret_cast<int *>(lists + p.at_cache_counters)};
-    STEP_TRY(launch_cache_attention(c, k_cache, v_cache, ctx->stream));
-  }
-  if (p.n_rows) {
-    uint16_t *kr = reinterpret_cast<uint16_t *>(ws + o_bytes + ml_bytes);
-    uint16_t *vr = reinterpret_cast<uint16_t *>(ws + o_bytes + ml_bytes + kv_bytes);
+  auto args = [&](const StepPlan::List &l) {
+    return StepAttnArgs{seq_view(b), reinterpret_cast<const AttnPiece *>(lists + l.at), l.n,
+                        reinterpret_cast<const _Float16 *>(q), reinterpret_cast<_Float16 *>(out), b->g.n_head,
+                        b->g.n_head_kv, b->g.head_dim, l.heads,
+                        Join{reinterpret_cast<float *>(ws) + l.rec * hd, reinterpret_cast<float2 *>(ws + o_bytes) + l.rec,
+                             reinterpret_cast<int *>(lists + l.counters)}};
+  };
+  for (int i = 0; i < 2; i++)
+    if (p.list[i].n) STEP_TRY(launch_cache_attention(args(p.list[i]), i + 1, k_cache, v_cache, ctx->stream));
+  if (p.list[2].n) {
     if (p.n_tiles) {
+      uint16_t *kr = reinterpret_cast<uint16_t *>(ws + o_bytes + ml_bytes), *vr = kr + kv_bytes / 2;
       STEP_TRY(launch_kv_load_paged(reinterpret_cast<const LoadTile *>(lists + p.at_tiles), p.n_tiles, seq_view(b).pages,
                                     b->g.page_size, (int)width, k_cache, v_cache, kr, vr, ctx->stream));
       k = kr;
       v = vr;
     }
-    StepAttnArgs r = base;
-    r.pieces = reinterpret_cast<const AttnPiece *>(lists + p.at_rows);
-    r.n_pieces = p.n_rows;
-    r.join = Join{rec_o + p.cache_rec * hd, rec_ml + p.cache_rec, reinterpret_cast<int *>(lists + p.at_row_counters)};
-    STEP_TRY(launch_row_attention(r, reinterpret_cast<const SeqKv *>(lists + p.at_kv), reinterpret_cast<const _Float16 *>(k),
-                                  reinterpret_cast<const _Float16 *>(v), ctx->stream));
+    STEP_TRY(launch_row_attention(args(p.list[2]), reinterpret_cast<const SeqKv *>(lists + p.at_kv),
+                                  reinterpret_cast<const _Float16 *>(k), reinterpret_cast<const _Float16 *>(v), ctx->stream));
   }
   return SULIMO_HIP_OK;
 }

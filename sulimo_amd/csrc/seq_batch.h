@@ -10,14 +10,21 @@ struct StepArray {
   void *dev = nullptr;
   size_t bytes = 0;
 };
-// The work lists of a step's attention (attention_step.hip), for the paged or the packed form.
+// The work lists of a step's attention (attention_step.hip), for the paged or the packed form:
+// pieces over the cache by 16 rows and by 32, and over f16 rows.
 struct StepPlan {
+  struct List {
+    int n = 0, heads = 1;         // pieces, KV heads of a workgroup
+    size_t at = 0, counters = 0;  // where in `lists` the pieces and their counters are
+    size_t rec = 0;               // first record row
+  };
   bool ready = false;
   StepArray lists;
-  int n_cache = 0, n_rows = 0, n_tiles = 0;  // pieces over the cache, pieces over f16 rows, load tiles
-  long read_rows = 0;                        // cache rows that are read back
-  size_t cache_rec = 0, rec_rows = 0;
-  size_t at_rows = 0, at_kv = 0, at_tiles = 0, at_cache_counters = 0, at_row_counters = 0;
+  List list[3];
+  size_t rec_rows = 0;
+  int n_tiles = 0;     // load tiles
+  long read_rows = 0;  // cache rows that are read back
+  size_t at_kv = 0, at_tiles = 0;
 };
 }  // namespace sulimo
 

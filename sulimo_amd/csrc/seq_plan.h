@@ -10,8 +10,9 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <math.h>
+
 #include <algorithm>
-#include <numeric>
 #include <string>
 #include <vector>
 
@@ -177,18 +178,27 @@ struct AttnSplit {
   int key_tile;  // positions
   int heads, sub;
   int slots;     // workgroups that run at once
+  int threads;   // of a workgroup
+  // microseconds: a piece's start and end, a step of sub key tiles, and one round of a join (8
+  // pieces of two times four values a thread)
+  double piece, step, join;
 };
 struct AttnPlan {
   std::vector<AttnPiece> pieces;
+  int heads = 1;        // KV heads of a workgroup
   int counters = 0;     // arrival counters (head groups of every split tile)
   size_t rec_rows = 0;  // record rows, each head_dim floats and (m, l)
+  double cost = 0;      // the time the cut was chosen for
 };
 inline int first_seen(const SeqShape &g, int pos) { return g.window && pos >= g.window ? pos - g.window + 1 : 0; }
 
-// The row tiles of the sequences in `which`, cut so that their workgroups run in as few rounds
-// of `slots` as the uncut tiles would need: the smallest piece that keeps to that.
+// The row tiles of the sequences in `which`, cut into pieces of at most C steps. Pieces that all
+// run at once take the longest one's time; more of them, at best their share of the slots, and
+// half a piece for the last ones' unevenness. A cut tile's join comes behind that. C is the one
+// of least time.
 inline AttnPlan plan_attention_pieces(const SeqShape &g, const Seqs &q, const std::vector<int> &which, const AttnSplit &a) {
   AttnPlan plan;
+  plan.heads = a.heads;
   const int G = g.n_head / g.n_head_kv, groups = g.n_head_kv / a.heads;
   struct Tile {
     int seq, row0, live, t0, t1, steps;
@@ -207,18 +217,31 @@ inline AttnPlan plan_attention_pieces(const SeqShape &g, const Seqs &q, const st
     }
   }
   if (tiles.empty()) return plan;
-  const long per_round = std::max(1, a.slots / groups);
-  const long limit = ((long)tiles.size() + per_round - 1) / per_round * per_round;
-  auto fits = [&](int C) {
+  const int slots = std::max(1, a.slots / groups);
+  auto cost = [&](int C) {
     long n = 0;
-    for (const Tile &t : tiles) n += (t.steps + C - 1) / C;
-    return n <= limit;
+    double total = 0, join = 0;
+    for (const Tile &t : tiles) {
+      const int np = (t.steps + C - 1) / C;
+      n += np;
+      total += np * a.piece + t.steps * a.step;
+      if (np > 1)
+        join = std::max(join, a.join * ((np + 7) / 8) * std::ceil(a.heads * t.live * (g.head_dim / 4) / (2.0 * a.threads)));
+    }
+    const double one = a.piece + a.step * C;
+    return (n <= slots ? one : std::max(one, total / slots) + one / 2) + join;
   };
-  int C = 1;
-  for (int hi = most; C < hi;) {  // C = most fits: one piece a tile
-    const int mid = C + (hi - C) / 2;
-    if (fits(mid)) hi = mid;
-    else C = mid + 1;
+  int C = most, last = most;
+  plan.cost = cost(most);
+  for (int np = 2; np <= 64 && last > 1; np++) {
+    const int c = (most + np - 1) / np;
+    if (c == last) continue;
+    last = c;
+    const double t = cost(c);
+    if (t < plan.cost) {
+      plan.cost = t;
+      C = c;
+    }
   }
   for (const Tile &t : tiles) {
     const int np = (t.steps + C - 1) / C;
@@ -242,18 +265,28 @@ inline AttnPlan plan_attention_pieces(const SeqShape &g, const Seqs &q, const st
 }
 
 // Few rows read the Q8_0 cache directly (attention_cache.hip): 8 waves, of which 8 / heads share
-// a KV head and take every (8 / heads)th key tile.
-constexpr int kCacheRows = 32, kCacheWaves = 8;
-inline int cache_heads(int n_head_kv) {  // the largest power of two up to 8 that divides
-  return n_head_kv % 8 == 0 ? 8 : n_head_kv % 4 == 0 ? 4 : n_head_kv % 2 == 0 ? 2 : 1;
+// a KV head and take every (8 / heads)th key tile, row_tiles times 16 rows each.
+constexpr int kCacheWaves = 8;
+inline AttnSplit cache_split(const SeqShape &g, int row_tiles, int heads, int cus) {
+  return AttnSplit{16 * row_tiles, g.head_dim == 128 ? 32 : 64, heads, kCacheWaves / heads, cus, 64 * kCacheWaves,
+                   5.5, row_tiles == 1 ? 2.8 : 4.0, 1.8};
 }
-inline AttnSplit cache_split(const SeqShape &g, int cus) {
-  const int heads = cache_heads(g.n_head_kv);
-  return AttnSplit{kCacheRows, g.head_dim == 128 ? 32 : 64, heads, kCacheWaves / heads, cus};
+// The KV heads of a workgroup: eight keep every line of the cache's rows in one workgroup; fewer,
+// with more waves a head, have less to join where there is little to do.
+inline AttnPlan plan_cache_attention(const SeqShape &g, const Seqs &q, const std::vector<int> &which, int row_tiles, int cus) {
+  AttnPlan best;
+  bool any = false;
+  for (int heads = 8; heads >= 1; heads /= 2) {
+    if (g.n_head_kv % heads) continue;
+    AttnPlan p = plan_attention_pieces(g, q, which, cache_split(g, row_tiles, heads, cus));
+    if (!any || p.cost < best.cost) best = std::move(p);
+    any = true;
+  }
+  return best;
 }
 // Many rows read f16 keys and values (attention_rows.hip), the cache's read back first.
 constexpr int kRowTile = 128, kRowKeys = 64;
-inline AttnSplit row_split(int cus) { return AttnSplit{kRowTile, kRowKeys, 1, 1, 2 * cus}; }
+inline AttnSplit row_split(int cus) { return AttnSplit{kRowTile, kRowKeys, 1, 1, 2 * cus, 256, 4.0, 1.5, 1.8}; }
 
 // Where a sequence's f16 keys and values lie: position p in [lo, lo + len) is row row0 + p - lo.
 struct SeqKv {

@@ -23,9 +23,10 @@ struct StepAttnArgs {
   const _Float16 *q;  // [rows][n_head][head_dim]
   _Float16 *out;
   int n_head, n_head_kv, head_dim;
+  int heads;  // KV heads of a workgroup
   Join join;
 };
-int32_t launch_cache_attention(const StepAttnArgs &c, const uint8_t *k_cache, const uint8_t *v_cache, hipStream_t s);
+int32_t launch_cache_attention(const StepAttnArgs &c, int row_tiles, const uint8_t *k_cache, const uint8_t *v_cache, hipStream_t s);
 // kv: where each sequence's f16 keys and values lie in k and v ([rows][n_head_kv][head_dim])
 int32_t launch_row_attention(const StepAttnArgs &c, const SeqKv *kv, const _Float16 *k, const _Float16 *v, hipStream_t s);
 
@@ -34,6 +35,7 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef short short8v __attribute__((ext_vector_type(8)));
@@ -43,14 +45,15 @@ constexpr float kLazy = 8.0f;  // log2 growth of the running max before O is res
 
 __device__ __forceinline__ half2v as_h2(uint32_t v) { return __builtin_bit_cast(half2v, v); }
 
-// Device-scope (sc1) stores and loads: coherent across the XCDs' L2 caches by themselves.
+// Device-scope (sc1) store: past this XCD's L2 cache, to where the other XCDs see it.
 __device__ __forceinline__ void st_dev(float2 *p, float2 v) {
   __hip_atomic_store(reinterpret_cast<uint64_t *>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
                      __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float2 ld_dev(const float2 *p) {
-  return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<uint64_t *>(const_cast<float2 *>(p)),
-                                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+
+// The same for four floats at a 16-byte aligned address; whoever waits for it waits for vmcnt.
+__device__ __forceinline__ void st_dev4(float *p, floatx4 v) {
+  asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
 }
 
 // max over lanes l and l ^ 32
@@ -69,17 +72,6 @@ __device__ __forceinline__ half8 read_tr(const char *p, const char *q) {
   return __builtin_bit_cast(half8, z);
 }
 
-// O^T tile i (dimensions 32 i .. + 31) of a lane's row to record row rr.
-template <int HD>
-__device__ __forceinline__ void record_tile(const Join &j, size_t rr, int i, int lg, const floatx16 &o) {
-  float2 *dst = reinterpret_cast<float2 *>(j.o + rr * HD) + 16 * i + 2 * lg;
-#pragma unroll
-  for (int g = 0; g < 4; g++) {
-    st_dev(dst + 4 * g, float2{o[4 * g], o[4 * g + 1]});
-    st_dev(dst + 4 * g + 1, float2{o[4 * g + 2], o[4 * g + 3]});
-  }
-}
-
 // After a workgroup stored its piece's records: whether it is the tile's last one (for head
 // group `group`). Every thread of the workgroup calls it.
 __device__ __forceinline__ bool arrived_last(const Join &j, const AttnPiece &pc, int group, int *shared) {
@@ -96,54 +88,75 @@ __device__ __forceinline__ bool arrived_last(const Join &j, const AttnPiece &pc,
 }
 
 // Joins the pieces of a row tile for heads KV heads from head0 on, in piece order: four values
-// of one (head, row) a thread. out: the sequence's first row.
+// of one (head, row) a job, kJobs jobs of a thread at a time with kPieces pieces' loads of each in
+// flight. out: the sequence's first row.
 template <int HD, int THREADS>
 __device__ __forceinline__ void join_pieces(const Join &j, const AttnPiece &pc, int head0, int heads, int live,
                                             int n_head, int n_head_kv, _Float16 *out) {
-  const int G = n_head / n_head_kv, rows = heads * live;
-  for (int job = threadIdx.x; job < rows * (HD / 4); job += THREADS) {
-    const int hr = job / (HD / 4), e = job % (HD / 4);
-    const int hh = head0 + hr / live, row = pc.row0 + hr % live;
-    const size_t r0 = (size_t)pc.rec + (size_t)hh * live + hr % live, stride = (size_t)n_head_kv * live;
-    float m = -INFINITY, l = 0.0f;
-    float4 acc{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int B = 8;  // pieces whose loads are in flight together
-    for (int p0 = 0; p0 < pc.n_pieces; p0 += B) {
-      float2 ml[B], x[B], y[B];
+  // the records were stored past the L2 caches: nothing older may be read from this one
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  constexpr int kJobs = 2, kPieces = 8;
+  const int G = n_head / n_head_kv, jobs = heads * live * (HD / 4);
+  const size_t stride = (size_t)n_head_kv * live;
+  for (int job0 = threadIdx.x; job0 < jobs; job0 += THREADS * kJobs) {
+    float m[kJobs], l[kJobs];
+    float4 acc[kJobs];
+    size_t r0[kJobs];
 #pragma unroll
-      for (int b = 0; b < B; b++) {
-        const size_t rr = r0 + min(p0 + b, pc.n_pieces - 1) * stride;
-        const float2 *src = reinterpret_cast<const float2 *>(j.o + rr * HD) + 2 * e;
-        ml[b] = ld_dev(j.ml + rr);
-        x[b] = ld_dev(src);
-        y[b] = ld_dev(src + 1);
-      }
-      float mn = m;
+    for (int x = 0; x < kJobs; x++) {
+      m[x] = -INFINITY;
+      l[x] = 0.0f;
+      acc[x] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+      r0[x] = (size_t)pc.rec + (size_t)head0 * live + min(job0 + x * THREADS, jobs - 1) / (HD / 4);  // (head, row)
+    }
+    const int e = job0 % (HD / 4);  // the same for all: THREADS is a multiple
+    static_assert(THREADS % (HD / 4) == 0, "jobs of a thread are at one place of their rows");
+    for (int p0 = 0; p0 < pc.n_pieces; p0 += kPieces) {
+      float2 ml[kJobs][kPieces];
+      float4 v[kJobs][kPieces];
 #pragma unroll
-      for (int b = 0; b < B; b++) mn = fmaxf(mn, ml[b].x);
-      const float ms = mn == -INFINITY ? 0.0f : mn;
-      const float old = __builtin_amdgcn_exp2f(m - ms);
-      m = mn;
-      l *= old;
-      acc.x *= old;
-      acc.y *= old;
-      acc.z *= old;
-      acc.w *= old;
+      for (int x = 0; x < kJobs; x++)
 #pragma unroll
-      for (int b = 0; b < B; b++) {
-        if (p0 + b >= pc.n_pieces) continue;
-        const float w = __builtin_amdgcn_exp2f(ml[b].x - ms);
-        l += ml[b].y * w;
-        acc.x += x[b].x * w;
-        acc.y += x[b].y * w;
-        acc.z += y[b].x * w;
-        acc.w += y[b].y * w;
+        for (int b = 0; b < kPieces; b++) {
+          const size_t rr = r0[x] + min(p0 + b, pc.n_pieces - 1) * stride;
+          ml[x][b] = j.ml[rr];
+          v[x][b] = reinterpret_cast<const float4 *>(j.o + rr * HD)[e];
+        }
+#pragma unroll
+      for (int x = 0; x < kJobs; x++) {
+        float mn = m[x];
+#pragma unroll
+        for (int b = 0; b < kPieces; b++) mn = fmaxf(mn, ml[x][b].x);
+        const float ms = mn == -INFINITY ? 0.0f : mn;
+        const float old = __builtin_amdgcn_exp2f(m[x] - ms);
+        m[x] = mn;
+        l[x] *= old;
+        acc[x].x *= old;
+        acc[x].y *= old;
+        acc[x].z *= old;
+        acc[x].w *= old;
+#pragma unroll
+        for (int b = 0; b < kPieces; b++) {
+          if (p0 + b >= pc.n_pieces) continue;
+          const float w = __builtin_amdgcn_exp2f(ml[x][b].x - ms);
+          l[x] += ml[x][b].y * w;
+          acc[x].x += v[x][b].x * w;
+          acc[x].y += v[x][b].y * w;
+          acc[x].z += v[x][b].z * w;
+          acc[x].w += v[x][b].w * w;
+        }
       }
     }
-    const float inv = 1.0f / l;
-    const int t = row / G, head = hh * G + row % G;
-    *reinterpret_cast<half4 *>(out + ((size_t)t * n_head + head) * HD + 4 * e) =
-        half4{(_Float16)(acc.x * inv), (_Float16)(acc.y * inv), (_Float16)(acc.z * inv), (_Float16)(acc.w * inv)};
+#pragma unroll
+    for (int x = 0; x < kJobs; x++) {
+      const int job = job0 + x * THREADS;
+      if (job >= jobs) continue;
+      const float inv = 1.0f / l[x];
+      const int hr = job / (HD / 4), row = pc.row0 + hr % live;
+      const int t = row / G, head = (head0 + hr / live) * G + row % G;
+      *reinterpret_cast<half4 *>(out + ((size_t)t * n_head + head) * HD + 4 * e) = half4{
+          (_Float16)(acc[x].x * inv), (_Float16)(acc[x].y * inv), (_Float16)(acc[x].z * inv), (_Float16)(acc[x].w * inv)};
+    }
   }
 }
 

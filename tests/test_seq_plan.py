@@ -53,7 +53,7 @@ extern "C" void pieces(int heads, int kv_heads, int hd, int window, size_t n, co
   plan_seqs(g, n, nn, st, nullptr, 0, &q);
   std::vector<int> all(n);
   for (size_t s = 0; s < n; s++) all[s] = (int)s;
-  const AttnPlan p = plan_attention_pieces(g, q, all, AttnSplit{rows, key_tile, group_heads, sub, slots});
+  const AttnPlan p = plan_attention_pieces(g, q, all, AttnSplit{rows, key_tile, group_heads, sub, slots, 256, 5.0, 2.0, 3.0});
   memcpy(out, p.pieces.data(), p.pieces.size() * sizeof(AttnPiece));
   sizes[0] = p.pieces.size();
   sizes[1] = (size_t)p.counters;
@@ -63,7 +63,6 @@ extern "C" uint32_t divided(uint32_t p, uint32_t d) {
   const FastDiv f = fast_div(d);
   return (uint32_t)(((uint64_t)p * f.magic) >> f.shift);
 }
-extern "C" int heads_of(int hk) { return cache_heads(hk); }
 '''
 
 
@@ -186,7 +185,7 @@ def test_lengths_that_are_no_lengths_raise(bad):
         hip._u32(bad, (1,))
 
 
-@pytest.mark.parametrize("rows,key_tile,heads,sub", [(32, 32, 8, 1), (32, 32, 2, 4), (32, 64, 1, 8), (128, 64, 1, 1)])
+@pytest.mark.parametrize("rows,key_tile,heads,sub", [(16, 32, 8, 1), (32, 32, 2, 4), (16, 64, 1, 8), (128, 64, 1, 1)])
 @pytest.mark.parametrize("slots", [1, 40, 256, 512])
 @pytest.mark.parametrize("window", [0, 1, 100])
 @pytest.mark.parametrize("new,start", [([1], [0]), ([1], [5000]), ([1, 0, 7, 200], [3, 9, 4000, 70]), ([1] * 300, list(range(300))),
@@ -224,8 +223,6 @@ def test_pieces_cover_every_key_once(lib, rows, key_tile, heads, sub, slots, win
             recs.append((ps[0][4], ps[0][4] + len(ps) * Hk * live))
     recs.sort()
     assert all(a[1] <= b[0] for a, b in zip(recs, recs[1:])) and (not recs or recs[-1][1] <= rec_rows)
-    per_round = max(1, slots // (Hk // heads))
-    assert n <= -(-len(want) // per_round) * per_round
 
 
 def test_division_by_the_page_size(lib):
@@ -234,9 +231,3 @@ def test_division_by_the_page_size(lib):
         for p in [0, 1, d - 1, d, d + 1, 2 * d - 1, 2 * d, 2**31 - 1, 2**31 - 2] + [int(x) for x in rng.integers(0, 2**31, 200)]:
             if p < 2**31:
                 assert lib.divided(p, d) == p // d, (p, d)
-
-
-def test_heads_of_a_workgroup(lib):
-    for hk in range(1, 65):
-        h = lib.heads_of(hk)
-        assert h in (1, 2, 4, 8) and hk % h == 0 and (h == 8 or hk % (2 * h) != 0)
