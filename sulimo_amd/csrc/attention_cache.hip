@@ -33,6 +33,8 @@
 // order, so the result does not depend on who that is.
 #include <math.h>
 
+#include <type_traits>
+
 #include "step_attn.h"
 
 namespace sulimo {
@@ -134,7 +136,9 @@ __global__ __launch_bounds__(64 * kCacheWaves, 2) void cache_attn_kernel(CacheAt
   constexpr int RD = HD == 128 ? 34 : 19;                // dwords of a raw row in LDS: reads of 32 lanes meet in no bank
   constexpr int ROW = HD == 128 ? 288 : 144;             // LDS bytes of a V row
   constexpr int OROW = HD + 4;                           // floats of a row of sums in LDS
-  constexpr int WB = KT * ROW > 16 * RT * OROW * 4 ? KT * ROW : 16 * RT * OROW * 4;  // LDS bytes of a wave
+  constexpr bool QLDS = RT > 1;  // Q^T of two row tiles is read from LDS: in registers, loads in flight would spill
+  constexpr int WT = KT * ROW + (QLDS ? RT * QS * 1024 : 0);
+  constexpr int WB = WT > 16 * RT * OROW * 4 ? WT : 16 * RT * OROW * 4;  // LDS bytes of a wave
   static_assert(KT * ROW >= KT * RD * 4 + 512, "a wave's LDS also holds raw rows");
   __shared__ __attribute__((aligned(16))) char lds[kCacheWaves][WB];
   __shared__ float2 lml[kCacheWaves][16 * RT];
@@ -153,27 +157,35 @@ __global__ __launch_bounds__(64 * kCacheWaves, 2) void cache_attn_kernel(CacheAt
   const float c = 1.4426950408889634f / sqrtf((float)HD);
   const int blk = HD == 128 ? (g >> 1) | (g & 1) << 1 : g & 1;  // the lane's block of a head
   const bool odd = blk & 1;
-  // dimension pair (of the block's 16) at position pair j
-  const int turn = odd ? 15 : 0;
 
   // Q^T (B operand) in the lanes' order of dimensions
+  char *mine = lds[wave];
   half8 qf[RT][QS];
+  auto q_at = [&](int x, int s) __attribute__((always_inline)) {
+    return reinterpret_cast<half8 *>(mine + KT * ROW + (x * QS + s) * 1024) + lane;
+  };
   int P[RT];
 #pragma unroll
   for (int x = 0; x < RT; x++) {
     const int r = pc.row0 + min(16 * x + r16, live - 1);  // dead rows repeat the last one
     const int t = r / G;
     P[x] = start + t;
-    const _Float16 *q = a.q + ((size_t)(off + t) * a.n_head + kvh * G + r % G) * HD + 32 * blk;
+    // the block's 16 dimension pairs, turned by one where positions are
+    const u32x4 *q = reinterpret_cast<const u32x4 *>(a.q + ((size_t)(off + t) * a.n_head + kvh * G + r % G) * HD + 32 * blk);
+    const u32x4 n0 = q[0], n1 = q[1], n2 = q[2], n3 = q[3];
+    const uint32_t n[16] = {n0[0], n0[1], n0[2], n0[3], n1[0], n1[1], n1[2], n1[3],
+                            n2[0], n2[1], n2[2], n2[3], n3[0], n3[1], n3[2], n3[3]};
 #pragma unroll
     for (int s = 0; s < QS; s++) {
-      const int ch = HD == 128 ? s : 2 * s + (g >> 1);
+      u32x4 y;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const half2v y = *reinterpret_cast<const half2v *>(q + 2 * ((4 * ch + e + turn) & 15));
-        qf[x][s][2 * e] = y[0];
-        qf[x][s][2 * e + 1] = y[1];
+        auto pair = [&](int j) { return odd ? n[(j + 15) & 15] : n[j]; };
+        if constexpr (HD == 128) y[e] = pair(4 * s + e);
+        else y[e] = g >> 1 ? pair(8 * s + 4 + e) : pair(8 * s + e);
       }
+      qf[x][s] = __builtin_bit_cast(half8, y);
+      if constexpr (QLDS) *q_at(x, s) = qf[x][s];
     }
   }
 
@@ -214,7 +226,6 @@ __global__ __launch_bounds__(64 * kCacheWaves, 2) void cache_attn_kernel(CacheAt
       }
     }
   };
-  char *mine = lds[wave];
   auto stage = [&](const Raw &x) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < kUnits; j++) {
@@ -256,7 +267,8 @@ __global__ __launch_bounds__(64 * kCacheWaves, 2) void cache_attn_kernel(CacheAt
       for (int m = 0; m < MT; m++) st[x][m] = floatx4{};
     auto product = [&](half8 k, int s, int m) __attribute__((always_inline)) {
 #pragma unroll
-      for (int x = 0; x < RT; x++) st[x][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[x][s], st[x][m], 0, 0, 0);
+      for (int x = 0; x < RT; x++)
+        st[x][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, QLDS ? *q_at(x, s) : qf[x][s], st[x][m], 0, 0, 0);
     };
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -429,29 +441,44 @@ __global__ __launch_bounds__(64 * kCacheWaves, 2) void cache_attn_kernel(CacheAt
   __syncthreads();
   // four dimensions of a row a thread
   const int w0 = wave - sw;
-  for (int job = 64 * sw + lane; job < live * (HD / 4); job += 64 * sub) {
-    const int row = job / (HD / 4), d = 4 * (job % (HD / 4));
-    float m = -INFINITY, l = 0.0f;
-    for (int j = 0; j < sub; j++) m = fmaxf(m, lml[w0 + j][row].x);
-    const float ms = m == -INFINITY ? 0.0f : m;
-    floatx4 acc{};
-    for (int j = 0; j < sub; j++) {
-      const float2 ml = lml[w0 + j][row];
-      const float f = __builtin_amdgcn_exp2f(ml.x - ms);
-      l += ml.y * f;
-      acc += *reinterpret_cast<const floatx4 *>(reinterpret_cast<const float *>(lds[w0 + j]) + row * OROW + d) * f;
+  auto add_up = [&](auto subs) __attribute__((always_inline)) {
+    constexpr int SUB = decltype(subs)::value;
+    for (int job = 64 * sw + lane; job < live * (HD / 4); job += 64 * SUB) {
+      const int row = job / (HD / 4), d = 4 * (job % (HD / 4));
+      float2 ml[SUB];
+      floatx4 part[SUB];
+#pragma unroll
+      for (int j = 0; j < SUB; j++) {
+        ml[j] = lml[w0 + j][row];
+        part[j] = *reinterpret_cast<const floatx4 *>(reinterpret_cast<const float *>(lds[w0 + j]) + row * OROW + d);
+      }
+      float m = ml[0].x, l = 0.0f;
+#pragma unroll
+      for (int j = 1; j < SUB; j++) m = fmaxf(m, ml[j].x);
+      const float ms = m == -INFINITY ? 0.0f : m;
+      floatx4 acc{};
+#pragma unroll
+      for (int j = 0; j < SUB; j++) {
+        const float f = __builtin_amdgcn_exp2f(ml[j].x - ms);
+        l += ml[j].y * f;
+        acc += part[j] * f;
+      }
+      if (pc.n_pieces == 1) {
+        const int r = pc.row0 + row;
+        const float inv = 1.0f / l;
+        *reinterpret_cast<half4 *>(a.out + ((size_t)(off + r / G) * a.n_head + kvh * G + r % G) * HD + d) =
+            half4{(_Float16)(acc[0] * inv), (_Float16)(acc[1] * inv), (_Float16)(acc[2] * inv), (_Float16)(acc[3] * inv)};
+      } else {
+        const size_t rr = (size_t)pc.rec + ((size_t)pc.piece * a.n_head_kv + kvh) * live + row;
+        st_dev4(a.join.o + rr * HD + d, acc);
+        if (d == 0) st_dev(a.join.ml + rr, float2{m, l});
+      }
     }
-    if (pc.n_pieces == 1) {
-      const int r = pc.row0 + row;
-      const float inv = 1.0f / l;
-      *reinterpret_cast<half4 *>(a.out + ((size_t)(off + r / G) * a.n_head + kvh * G + r % G) * HD + d) =
-          half4{(_Float16)(acc[0] * inv), (_Float16)(acc[1] * inv), (_Float16)(acc[2] * inv), (_Float16)(acc[3] * inv)};
-    } else {
-      const size_t rr = (size_t)pc.rec + ((size_t)pc.piece * a.n_head_kv + kvh) * live + row;
-      st_dev4(a.join.o + rr * HD + d, acc);
-      if (d == 0) st_dev(a.join.ml + rr, float2{m, l});
-    }
-  }
+  };
+  if (sub == 8) add_up(std::integral_constant<int, 8>{});
+  else if (sub == 4) add_up(std::integral_constant<int, 4>{});
+  else if (sub == 2) add_up(std::integral_constant<int, 2>{});
+  else add_up(std::integral_constant<int, 1>{});
   if (pc.n_pieces > 1 && arrived_last(a.join, pc, blockIdx.y, &last_one))
     join_pieces<HD, 64 * kCacheWaves>(a.join, pc, blockIdx.y * heads, heads, live, a.n_head, a.n_head_kv,
                                       a.out + (size_t)off * a.n_head * HD);

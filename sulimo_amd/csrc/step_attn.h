@@ -45,13 +45,18 @@ constexpr float kLazy = 8.0f;  // log2 growth of the running max before O is res
 
 __device__ __forceinline__ half2v as_h2(uint32_t v) { return __builtin_bit_cast(half2v, v); }
 
-// Device-scope (sc1) store: past this XCD's L2 cache, to where the other XCDs see it.
+// Device-scope (sc1) stores and loads: past this XCD's L2 cache, where the other XCDs see them.
+// (An acquire fence before plain loads empties the cache instead, and took 6 to 17 us.)
 __device__ __forceinline__ void st_dev(float2 *p, float2 v) {
   __hip_atomic_store(reinterpret_cast<uint64_t *>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
                      __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The same for four floats at a 16-byte aligned address; whoever waits for it waits for vmcnt.
+__device__ __forceinline__ float2 ld_dev(const float2 *p) {
+  return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<uint64_t *>(const_cast<float2 *>(p)),
+                                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+// The store of four floats at a 16-byte aligned address; whoever waits for it waits for vmcnt.
 __device__ __forceinline__ void st_dev4(float *p, floatx4 v) {
   asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
 }
@@ -93,8 +98,6 @@ __device__ __forceinline__ bool arrived_last(const Join &j, const AttnPiece &pc,
 template <int HD, int THREADS>
 __device__ __forceinline__ void join_pieces(const Join &j, const AttnPiece &pc, int head0, int heads, int live,
                                             int n_head, int n_head_kv, _Float16 *out) {
-  // the records were stored past the L2 caches: nothing older may be read from this one
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   constexpr int kJobs = 2, kPieces = 8;
   const int G = n_head / n_head_kv, jobs = heads * live * (HD / 4);
   const size_t stride = (size_t)n_head_kv * live;
@@ -119,8 +122,10 @@ __device__ __forceinline__ void join_pieces(const Join &j, const AttnPiece &pc, 
 #pragma unroll
         for (int b = 0; b < kPieces; b++) {
           const size_t rr = r0[x] + min(p0 + b, pc.n_pieces - 1) * stride;
-          ml[x][b] = j.ml[rr];
-          v[x][b] = reinterpret_cast<const float4 *>(j.o + rr * HD)[e];
+          ml[x][b] = ld_dev(j.ml + rr);
+          const float2 *o = reinterpret_cast<const float2 *>(j.o + rr * HD) + 2 * e;
+          const float2 o0 = ld_dev(o), o1 = ld_dev(o + 1);
+          v[x][b] = float4{o0.x, o0.y, o1.x, o1.y};
         }
 #pragma unroll
       for (int x = 0; x < kJobs; x++) {
