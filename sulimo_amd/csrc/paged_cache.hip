@@ -91,42 +91,73 @@ __global__ __launch_bounds__(256) void kv_store_paged_kernel(const int32_t *row_
   }
 }
 
-// grid.x: tiles of kLoadTile positions, grid.y: keys, values
+// grid.x: tiles of kLoadTile positions, grid.y: keys, values. The tile's cache rows are looked up
+// once, and four loads of a thread are in flight at a time (one at a time, each behind its own
+// look-up, read 12 conversations of 2000 to 8000 positions at 4.0 TB/s).
 __global__ __launch_bounds__(256) void kv_load_paged_kernel(const LoadTile *tiles, const int32_t *pages, int page_size,
                                                             int width, const uint8_t *k_cache, const uint8_t *v_cache,
                                                             _Float16 *k_out, _Float16 *v_out) {
+  __shared__ uint32_t slots[kLoadTile];
+  constexpr int kDeep = 4;
   const LoadTile t = tiles[blockIdx.x];
   const uint8_t *cache = blockIdx.y ? v_cache : k_cache;
   _Float16 *out = blockIdx.y ? v_out : k_out;
-  const uint32_t per_row = (uint32_t)width / 16, total = (uint32_t)t.count * per_row;
-  for (uint32_t i = threadIdx.x; i < total; i += 256) {  // four threads of a pair of blocks stay together
-    const uint32_t r = i / per_row, part = i - r * per_row;
-    const uint32_t p = (uint32_t)t.pos + r, pg = p / (uint32_t)page_size;
-    const size_t slot = (size_t)pages[t.page_off + pg] * page_size + (p - pg * (uint32_t)page_size);
-    const int j = part & 3;
-    const uint32_t *src = reinterpret_cast<const uint32_t *>(cache + (slot * (width / 32) + part / 2 - (j >> 1)) * 34);
-    const u32x4a4 w = *reinterpret_cast<const u32x4a4 *>(src + 4 * j + (j >> 1));
-    const uint32_t mid = src[8];
-    const uint32_t next = __shfl_down(w[0], 1, 64);
-    const uint32_t after = j ? mid : next;  // dword 4 for the first thread, 8 for the second
-    const uint32_t first = __shfl(w[0], (threadIdx.x & 63) & ~3, 64);
-    const float d = (float)__builtin_bit_cast(_Float16, (uint16_t)(j < 2 ? first : mid >> 16));
-    uint32_t c[4];
-    if (j < 2) {
-      c[0] = w[0] >> 16 | w[1] << 16;
-      c[1] = w[1] >> 16 | w[2] << 16;
-      c[2] = w[2] >> 16 | w[3] << 16;
-      c[3] = w[3] >> 16 | after << 16;
-    } else {
+  if ((int)threadIdx.x < t.count) {
+    const uint32_t p = (uint32_t)t.pos + threadIdx.x, pg = p / (uint32_t)page_size;
+    slots[threadIdx.x] = (uint32_t)pages[t.page_off + pg] * (uint32_t)page_size + (p - pg * (uint32_t)page_size);
+  }
+  __syncthreads();
+  const uint32_t per_row = (uint32_t)width / 16, count = (uint32_t)t.count;
+  const size_t row_bytes = (size_t)(width / 32) * 34;
+  const uint32_t step_row = 256 / per_row, step_part = 256 % per_row;
+  uint32_t row = threadIdx.x / per_row, part = threadIdx.x % per_row;
+  // the four threads of a pair of blocks have one row, and end together
+  for (;;) {
+    uint32_t r[kDeep], pt[kDeep], mid[kDeep];
+    u32x4a4 w[kDeep];
+    if (row >= count) break;
 #pragma unroll
-      for (int e = 0; e < 4; e++) c[e] = w[e];
+    for (int e = 0; e < kDeep; e++) {
+      r[e] = row;
+      pt[e] = part;
+      const int j = part & 3;
+      const uint32_t *src = reinterpret_cast<const uint32_t *>(cache + slots[min(row, count - 1)] * row_bytes +
+                                                               (size_t)(part / 2 - (j >> 1)) * 34);
+      w[e] = *reinterpret_cast<const u32x4a4 *>(src + 4 * j + (j >> 1));
+      mid[e] = src[8];
+      row += step_row;
+      part += step_part;
+      if (part >= per_row) {
+        part -= per_row;
+        row++;
+      }
     }
-    half8 o[2];
 #pragma unroll
-    for (int e = 0; e < 16; e++) o[e >> 3][e & 7] = (_Float16)((float)(int8_t)(c[e >> 2] >> (8 * (e & 3))) * d);
-    _Float16 *y = out + ((size_t)t.out_row + r) * width + part * 16;
-    *reinterpret_cast<half8 *>(y) = o[0];
-    *reinterpret_cast<half8 *>(y + 8) = o[1];
+    for (int e = 0; e < kDeep; e++) {
+      const int j = pt[e] & 3;
+      const uint32_t next = __shfl_down(w[e][0], 1, 64);
+      const uint32_t after = j ? mid[e] : next;  // dword 4 for the first thread, 8 for the second
+      const uint32_t first = __shfl(w[e][0], (threadIdx.x & 63) & ~3, 64);
+      const float d = (float)__builtin_bit_cast(_Float16, (uint16_t)(j < 2 ? first : mid[e] >> 16));
+      uint32_t c[4];
+      if (j < 2) {
+        c[0] = w[e][0] >> 16 | w[e][1] << 16;
+        c[1] = w[e][1] >> 16 | w[e][2] << 16;
+        c[2] = w[e][2] >> 16 | w[e][3] << 16;
+        c[3] = w[e][3] >> 16 | after << 16;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) c[i] = w[e][i];
+      }
+      half8 o[2];
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[i >> 3][i & 7] = (_Float16)((float)(int8_t)(c[i >> 2] >> (8 * (i & 3))) * d);
+      if (r[e] < count) {
+        _Float16 *y = out + ((size_t)t.out_row + r[e]) * width + pt[e] * 16;
+        *reinterpret_cast<half8 *>(y) = o[0];
+        *reinterpret_cast<half8 *>(y + 8) = o[1];
+      }
+    }
   }
 }
 

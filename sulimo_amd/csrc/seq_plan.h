@@ -30,7 +30,7 @@ struct Seqs {
 
 // Up to kLoadTile consecutive positions of one sequence, going to rows out_row .. of a
 // packed output.
-constexpr int kLoadTile = 64;
+constexpr int kLoadTile = 16;
 struct LoadTile {
   int32_t page_off, pos, out_row, count;
 };
