@@ -179,9 +179,10 @@ struct AttnSplit {
   int heads, sub;
   int slots;     // workgroups that run at once
   int threads;   // of a workgroup
-  // microseconds: a piece's start and end, a step of sub key tiles, and one round of a join (8
-  // pieces of two times four values a thread)
-  double piece, step, join;
+  // microseconds: a piece's start and end, what it takes longer with records, a step of sub key
+  // tiles where the slots are full and where few are taken, and one round of a join (8 pieces of
+  // two times four values a thread)
+  double piece, record, step, alone, join;
 };
 struct AttnPlan {
   std::vector<AttnPiece> pieces;
@@ -219,30 +220,44 @@ inline AttnPlan plan_attention_pieces(const SeqShape &g, const Seqs &q, const st
   if (tiles.empty()) return plan;
   const int slots = std::max(1, a.slots / groups);
   auto cost = [&](int C) {
-    long n = 0;
+    long n = 0, records = 0;
     double total = 0, join = 0;
     for (const Tile &t : tiles) {
       const int np = (t.steps + C - 1) / C;
       n += np;
-      total += np * a.piece + t.steps * a.step;
+      total += np * (a.piece + (np > 1 ? a.record : 0)) + t.steps * a.step;
+      if (np > 1) records += (long)np * g.n_head_kv * t.live;
       if (np > 1)
         join = std::max(join, a.join * ((np + 7) / 8) * std::ceil(a.heads * t.live * (g.head_dim / 4) / (2.0 * a.threads)));
     }
-    const double one = a.piece + a.step * C;
+    if (records > INT32_MAX) return HUGE_VAL;  // (AttnPiece.rec)
+    const double one = a.piece + (C < most ? a.record : 0) + std::max(a.alone, a.step * std::min(1.0, (double)n / slots)) * C;
     return (n <= slots ? one : std::max(one, total / slots) + one / 2) + join;
   };
-  int C = most, last = most;
+  int C = most;
   plan.cost = cost(most);
-  for (int np = 2; np <= 64 && last > 1; np++) {
-    const int c = (most + np - 1) / np;
-    if (c == last) continue;
-    last = c;
+  auto consider = [&](int c) {
     const double t = cost(c);
     if (t < plan.cost) {
       plan.cost = t;
       C = c;
     }
+  };
+  // the longest tile in 2 .. 64 equal pieces, and the shortest pieces that all run at once
+  for (int np = 2, last = most; np <= 64 && last > 1; np++) {
+    const int c = (most + np - 1) / np;
+    if (c != last) consider(c);
+    last = c;
   }
+  int lo = 1, hi = most;
+  while (lo < hi) {
+    const int c = (lo + hi) / 2;
+    long n = 0;
+    for (const Tile &t : tiles) n += (t.steps + c - 1) / c;
+    if (n <= slots) hi = c;
+    else lo = c + 1;
+  }
+  if (lo < most) consider(lo);
   for (const Tile &t : tiles) {
     const int np = (t.steps + C - 1) / C;
     AttnPiece p{t.seq, t.row0, 0, 0, 0, np, (int32_t)plan.rec_rows, plan.counters};
@@ -269,7 +284,7 @@ inline AttnPlan plan_attention_pieces(const SeqShape &g, const Seqs &q, const st
 constexpr int kCacheWaves = 8;
 inline AttnSplit cache_split(const SeqShape &g, int row_tiles, int heads, int cus) {
   return AttnSplit{16 * row_tiles, g.head_dim == 128 ? 32 : 64, heads, kCacheWaves / heads, cus, 64 * kCacheWaves,
-                   5.5, row_tiles == 1 ? 2.8 : 4.0, 1.8};
+                   5.5, 0.0, row_tiles == 1 ? 2.8 : 4.0, row_tiles == 1 ? 2.8 : 4.0, 1.8};
 }
 // The KV heads of a workgroup: eight keep every line of the cache's rows in one workgroup; fewer,
 // with more waves a head, have less to join where there is little to do.
@@ -285,8 +300,12 @@ inline AttnPlan plan_cache_attention(const SeqShape &g, const Seqs &q, const std
   return best;
 }
 // Many rows read f16 keys and values (attention_rows.hip), the cache's read back first.
+// A cut tile of 128 rows stores and joins 64 KiB a piece and head, which costs more than the
+// slots that it fills: 1000 tokens 27 us uncut and 49 in pieces of 2 tiles, 4096 tokens 126 and
+// 206, the eight prompts of 677 to 4000 tokens 285 and 420. A tile is cut where a chunk is short
+// and its history long.
 constexpr int kRowTile = 128, kRowKeys = 64;
-inline AttnSplit row_split(int cus) { return AttnSplit{kRowTile, kRowKeys, 1, 1, 2 * cus, 256, 4.0, 1.5, 1.8}; }
+inline AttnSplit row_split(int cus) { return AttnSplit{kRowTile, kRowKeys, 1, 1, 2 * cus, 256, 4.0, 24.0, 2.1, 1.2, 1.8}; }
 
 // Where a sequence's f16 keys and values lie: position p in [lo, lo + len) is row row0 + p - lo.
 struct SeqKv {

@@ -53,7 +53,7 @@ extern "C" void pieces(int heads, int kv_heads, int hd, int window, size_t n, co
   plan_seqs(g, n, nn, st, nullptr, 0, &q);
   std::vector<int> all(n);
   for (size_t s = 0; s < n; s++) all[s] = (int)s;
-  const AttnPlan p = plan_attention_pieces(g, q, all, AttnSplit{rows, key_tile, group_heads, sub, slots, 256, 5.0, 2.0, 3.0});
+  const AttnPlan p = plan_attention_pieces(g, q, all, AttnSplit{rows, key_tile, group_heads, sub, slots, 256, 5.0, 1.0, 2.0, 1.5, 3.0});
   memcpy(out, p.pieces.data(), p.pieces.size() * sizeof(AttnPiece));
   sizes[0] = p.pieces.size();
   sizes[1] = (size_t)p.counters;
