@@ -18,7 +18,10 @@ namespace {
 
 constexpr size_t align_up(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// Rows a KV head up to which a sequence's rows read the Q8_0 cache directly.
+// Rows a KV head up to which a sequence's rows read the Q8_0 cache directly; more have it read
+// back and go to the row kernel. Measured, 24 heads over 8, directly and by read-back: 126 rows of
+// one sequence behind 8000 positions 31 and 58 us, of 16 behind 4000 151 and 178, of 64 behind
+// 2000 288 and 296; 192 rows 43 and 57, 218 and 180, 479 and 407.
 constexpr int kDirectRows = 128;
 
 int32_t plan(sulimo_hip_seq_batch *b, bool packed) {
@@ -30,9 +33,9 @@ int32_t plan(sulimo_hip_seq_batch *b, bool packed) {
     const long rows = (long)b->q.n_new[s] * G;
     if (rows) which[packed || rows > kDirectRows ? 2 : rows > 16 ? 1 : 0].push_back(s);
   }
-  const AttnPlan a[3] = {plan_cache_attention(b->g, b->q, which[0], 1, cus),
-                         plan_cache_attention(b->g, b->q, which[1], 2, cus),
-                         plan_attention_pieces(b->g, b->q, which[2], row_split(cus))};
+  AttnPlan a[3];
+  plan_direct(b->g, b->q, which[0], which[1], cus, a);
+  a[2] = plan_attention_pieces(b->g, b->q, which[2], row_split(cus));
   std::vector<SeqKv> kv(b->q.n_seqs, SeqKv{0, 0, 0});
   std::vector<LoadTile> tiles;
   long rows = 0;
