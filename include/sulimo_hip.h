@@ -356,7 +356,8 @@ int32_t sulimo_hip_rope_table(sulimo_hip_ctx *ctx, size_t rope_dim, float freq_b
  *
  * The calls are asynchronous on the context's stream. A batch is used with the context it was
  * made with, by one thread at a time; it keeps device copies of its arrays and the workspace
- * of its calls. Buffers must be on the context's device. */
+ * of its calls; release it before the context. Buffers must be on the context's device, and one
+ * that a call writes must be none of its others unless it says so. */
 
 /* Head layout (head_dim 64 or 128, head_count % head_count_kv == 0), window (a query sees
  * its own and the window - 1 positions before it; 0: all before it) and cache shape of a
@@ -378,7 +379,8 @@ int32_t sulimo_hip_seq_batch_set(sulimo_hip_seq_batch *batch, size_t n_seqs, con
 /* Quantizes k and v, f16 [rows][head_count_kv * head_dim], into the pages of the new
  * positions, bytes as sulimo_hip_enqueue_kv_store writes them. k_values, v_values (f16, as k
  * and v; each may be NULL) receive f16(code * scale), what the cache now stands for: keys and
- * values for sulimo_hip_enqueue_attention_packed that agree with the cache. */
+ * values for sulimo_hip_enqueue_attention_packed that agree with the cache. k_values may be k,
+ * v_values may be v. */
 int32_t sulimo_hip_enqueue_kv_store_paged(sulimo_hip_ctx *ctx, const sulimo_hip_seq_batch *batch,
                                           const sulimo_hip_buffer *k, const sulimo_hip_buffer *v,
                                           sulimo_hip_buffer *k_cache, sulimo_hip_buffer *v_cache,

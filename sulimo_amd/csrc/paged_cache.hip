@@ -42,14 +42,15 @@ __global__ __launch_bounds__(256) void kv_store_paged_kernel(const int32_t *row_
   const uint32_t part = (uint32_t)(gid - row64 * per_row);
   const _Float16 *x = src + row64 * width + part * 16;
   const half8 a = *reinterpret_cast<const half8 *>(x), b = *reinterpret_cast<const half8 *>(x + 8);
-  float f[16], amax = 0.0f;
+  float f[16];
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     f[e] = (float)a[e];
     f[8 + e] = (float)b[e];
   }
+  float amax = fabsf(f[0]);  // (a block of nothing but NaN has a NaN scale, as in the ring)
 #pragma unroll
-  for (int e = 0; e < 16; e++) amax = fmaxf(amax, fabsf(f[e]));
+  for (int e = 1; e < 16; e++) amax = fmaxf(amax, fabsf(f[e]));
   amax = fmaxf(amax, __shfl_xor(amax, 1, 64));
   const float d = amax / 127.0f;
   const float id = d != 0.0f ? 1.0f / d : 0.0f;

@@ -5,6 +5,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <new>
 #include <string>
 
@@ -67,6 +68,13 @@ int32_t need(const sulimo_hip_ctx *ctx, const sulimo_hip_buffer *b, size_t bytes
   if (b->bytes < bytes)
     return fail(kInval, std::string(name) + " buffer holds " + std::to_string(b->bytes) + " bytes, needs " +
                             std::to_string(bytes));
+  return SULIMO_HIP_OK;
+}
+
+// A buffer that a call writes is none of its others.
+int32_t alone(const sulimo_hip_buffer *b, std::initializer_list<const sulimo_hip_buffer *> others, const char *name) {
+  for (const sulimo_hip_buffer *o : others)
+    if (b && b == o) return fail(kInval, std::string(name) + " is also another buffer of the call");
   return SULIMO_HIP_OK;
 }
 
@@ -160,7 +168,11 @@ int32_t sulimo_hip_enqueue_kv_store_paged(sulimo_hip_ctx *ctx, const sulimo_hip_
     STEP_TRY(need(ctx, v_cache, cache_bytes(b), "v_cache"));
     if (k_values) STEP_TRY(need(ctx, k_values, bytes, "k_values"));
     if (v_values) STEP_TRY(need(ctx, v_values, bytes, "v_values"));
-    if (k_cache == v_cache) return fail(kInval, "keys and values need a cache each");
+    STEP_TRY(alone(k_cache, {k, v, v_cache}, "k_cache"));
+    STEP_TRY(alone(v_cache, {k, v}, "v_cache"));
+    // (a thread reads its elements of k before it writes them)
+    STEP_TRY(alone(k_values, {v, k_cache, v_cache, v_values}, "k_values"));
+    STEP_TRY(alone(v_values, {k, k_cache, v_cache}, "v_values"));
     if (b->q.rows == 0) return SULIMO_HIP_OK;
     wrote(k_cache);
     wrote(v_cache);
@@ -183,7 +195,8 @@ int32_t sulimo_hip_enqueue_kv_load_paged(sulimo_hip_ctx *ctx, sulimo_hip_seq_bat
     STEP_TRY(need(ctx, v_cache, cache_bytes(b), "v_cache"));
     STEP_TRY(need(ctx, k_out, bytes, "k_out"));
     STEP_TRY(need(ctx, v_out, bytes, "v_out"));
-    if (k_out == v_out) return fail(kInval, "keys and values need an output each");
+    STEP_TRY(alone(k_out, {k_cache, v_cache, v_out}, "k_out"));
+    STEP_TRY(alone(v_out, {k_cache, v_cache}, "v_out"));
     if (b->q.positions == 0) return SULIMO_HIP_OK;
     if (!b->load_ready) {
       const std::vector<LoadTile> tiles = load_tiles(b->q);
@@ -212,7 +225,7 @@ int32_t sulimo_hip_enqueue_attention_paged(sulimo_hip_ctx *ctx, sulimo_hip_seq_b
     STEP_TRY(need(ctx, k_cache, cache_bytes(b), "k_cache"));
     STEP_TRY(need(ctx, v_cache, cache_bytes(b), "v_cache"));
     STEP_TRY(need(ctx, out, bytes, "out"));
-    if (out == q) return fail(kInval, "attention does not run in place");
+    STEP_TRY(alone(out, {q, k_cache, v_cache}, "out"));
     if (b->q.rows == 0) return SULIMO_HIP_OK;
     wrote(out);
     return attention_paged(b, dp<const uint16_t>(q), dp<const uint8_t>(k_cache), dp<const uint8_t>(v_cache),
@@ -234,7 +247,7 @@ int32_t sulimo_hip_enqueue_attention_packed(sulimo_hip_ctx *ctx, sulimo_hip_seq_
     STEP_TRY(need(ctx, k, kv, "k"));
     STEP_TRY(need(ctx, v, kv, "v"));
     STEP_TRY(need(ctx, out, bytes, "out"));
-    if (out == q || out == k || out == v) return fail(kInval, "attention does not run in place");
+    STEP_TRY(alone(out, {q, k, v}, "out"));
     if (b->q.rows == 0) return SULIMO_HIP_OK;
     wrote(out);
     return attention_packed(b, dp<const uint16_t>(q), dp<const uint16_t>(k), dp<const uint16_t>(v),
@@ -261,8 +274,8 @@ int32_t sulimo_hip_enqueue_verify_drafts(sulimo_hip_ctx *ctx, sulimo_hip_seq_bat
     if (temperature > 0.0f) STEP_TRY(need(ctx, uniforms, rows * 4, "uniforms"));
     STEP_TRY(need(ctx, accepted, (size_t)b->q.n_seqs * 4, "accepted"));
     STEP_TRY(need(ctx, answer, rows * 4, "answer"));
-    if (accepted == answer || answer == tokens || accepted == tokens)
-      return fail(kInval, "tokens, accepted and answer are three buffers");
+    STEP_TRY(alone(accepted, {logits, tokens, draft_probs, uniforms, answer}, "accepted"));
+    STEP_TRY(alone(answer, {logits, tokens, draft_probs, uniforms}, "answer"));
     if (rows == 0) return SULIMO_HIP_OK;
     wrote(accepted);
     wrote(answer);

@@ -447,6 +447,8 @@ class SeqBatch:
     def set(self, n_new, start_pos=None, page_table=None):
         """n_new, start_pos (None: all zero): one whole number per sequence; page_table
         [n_seqs][pages] (None: the step uses no cache)."""
+        if not self.ctx.handle:
+            raise HipError(ERR_INVALID_ARGUMENT, "the batch's context was released")
         n = len(n_new)
         new = _u32(n_new, (n,))
         start = _u32(start_pos, (n,)) if start_pos is not None else None

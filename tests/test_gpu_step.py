@@ -151,6 +151,35 @@ def test_store_writes_the_rings_bytes(ctx):
     assert np.array_equal(k.download(np.uint8, zero.shape), want) and np.array_equal(v.download(np.uint8, zero.shape), want)
 
 
+def test_store_of_what_is_not_finite_writes_the_rings_bytes(ctx):
+    """Blocks with infinities and NaN among their values, and with nothing else."""
+    rng = np.random.default_rng(31)
+    n, width = 16, 128
+    x = randn16(rng, n, width)
+    x[1, 5], x[2, 40], x[3, 70], x[4, 3] = np.inf, -np.inf, np.nan, np.inf
+    x[4, 4], x[5, :32], x[6, 32:64], x[7] = np.nan, np.nan, np.inf, -np.inf
+    batch = hip.SeqBatch(ctx, 2, 1, 128, page_size=n, n_pages=1)
+    batch.set([n], [0], [[0]])
+    zero = np.zeros((n, width // 32 * 34), np.uint8)
+    k, v, ring, xb = up(ctx, zero), up(ctx, zero), up(ctx, zero), up(ctx, x)
+    hip.enqueue_kv_store_paged(ctx, batch, xb, xb, k, v)
+    hip.enqueue_kv_store(ctx, xb, ring, 0, n, width // 32, n)
+    assert np.array_equal(k.download(np.uint8, zero.shape), ring.download(np.uint8, zero.shape))
+
+
+def test_store_in_place(ctx):
+    """k_values and v_values may be k and v."""
+    rng = np.random.default_rng(32)
+    n, width = 77, 192
+    x = [randn16(rng, n, width) for _ in range(2)]
+    batch = hip.SeqBatch(ctx, 3, 3, 64, page_size=16, n_pages=5)
+    batch.set([n], [0], [[3, 1, 0, 4, 2]])
+    kv, cache = [up(ctx, a) for a in x], [hip.HipBuffer.device_only(ctx, 80 * width // 32 * 34) for _ in range(2)]
+    hip.enqueue_kv_store_paged(ctx, batch, *kv, *cache, *kv)
+    for b, a in zip(kv, x):
+        assert np.array_equal(b.download(np.float16, a.shape).view(np.uint16), R.quantize(a)[1].view(np.uint16))
+
+
 @pytest.mark.parametrize("heads", HEADS)
 @pytest.mark.parametrize("start,new,page", CACHE)
 def test_load(ctx, heads, start, new, page):
@@ -213,6 +242,85 @@ def test_attention_hides_what_is_not_finite(ctx):
             want, bound = st.reference()
             check(got[:n - 1], want[:n - 1], bound[:n - 1])
             assert not np.any(np.isfinite(got[n - 1]))
+
+
+def test_a_cache_past_four_gigabytes(ctx):
+    """Pages whose bytes lie past 2^32 hold and give what those at the front do, for single tokens, a
+    short chunk and one that is read back."""
+    rng = np.random.default_rng(33)
+    H, Hk, hd, page, pages = 24, 8, 128, 64, 64000
+    width, S = Hk * hd, 3
+    assert pages * page * (width // 32) * 34 > 1 << 32
+    start, new = [0, 0, 0], [260, 300, 333]
+    k, v = (randn16(rng, sum(new), width) for _ in range(2))
+    kv = up(ctx, k), up(ctx, v)
+    steps = [([259, 290, 250], [1, 10, 83]), (start, new)]
+    q = [randn16(rng, sum(n), H, hd) for _, n in steps]
+    cache = [hip.HipBuffer.device_only(ctx, pages * page * (width // 32) * 34) for _ in range(2)]
+    answers = []
+    for first in (0, pages - 18):
+        table = first + np.arange(18, dtype=np.uint32).reshape(3, 6)[:, ::-1]
+        batch = hip.SeqBatch(ctx, H, Hk, hd, 0, page, pages)
+        batch.set(new, start, table)
+        hip.enqueue_kv_store_paged(ctx, batch, *kv, *cache)
+        out = [hip.HipBuffer.device_only(ctx, k.nbytes) for _ in range(2)]
+        hip.enqueue_kv_load_paged(ctx, batch, *cache, *out)
+        got = [b.download(np.float16, k.shape) for b in out]
+        for x, y in zip(got, (k, v)):
+            assert np.array_equal(x.view(np.uint16), R.quantize(y)[1].view(np.uint16))
+        for (st, n), x in zip(steps, q):
+            batch.set(n, st, table)
+            o = hip.HipBuffer.device_only(ctx, x.nbytes)
+            hip.enqueue_attention_paged(ctx, batch, up(ctx, x), *cache, o)
+            got.append(o.download(np.float16, x.shape))
+        answers.append(got)
+        batch.release()
+    for a, b in zip(*answers):
+        assert np.array_equal(a.view(np.uint16), b.view(np.uint16))
+    assert np.isfinite(answers[0][2]).all() and np.abs(answers[0][3]).max() > 0
+
+
+@pytest.mark.parametrize("new", [1, 20, 90])
+def test_pages_behind_the_window_may_stand_for_anything(ctx, new):
+    """A table's entries behind the window may all name one page that another sequence filled."""
+    rng = np.random.default_rng([34, new])
+    x = Step(ctx, rng, (24, 8, 128), [700, 300], [new, new], 16, window=100)
+    want = x.attend()
+    table = x.table.copy()
+    for s, a in enumerate(x.start):
+        table[s, :(a - 100 + 1) // 16] = x.pages - 1  # a spare page: NaN scales and wild codes
+    assert not (table == x.table).all()
+    x.batch.set(x.new, x.start, table)
+    assert np.array_equal(x.attend().view(np.uint16), want.view(np.uint16))
+    check(want[:-3], *x.reference())
+
+
+def test_contexts_and_batches_that_grow_and_shrink(ctx):
+    """Two contexts in turn without a wait, each with a batch that grows, shrinks and grows."""
+    other = hip.HipContext.new(0)
+    jobs, outs = [], []
+    for i, (n_seqs, new) in enumerate([(1, 1), (40, 3), (2, 100), (1, 1), (64, 1), (3, 400)]):
+        for c in (ctx, other):
+            jobs.append(Step(c, np.random.default_rng([35, i]), (4, 2, 64), [(37 * j) % 900 for j in range(n_seqs)],
+                             [new] * n_seqs, 32))
+    own = {id(c): hip.SeqBatch(c, 4, 2, 64, 0, 32, max(j.pages for j in jobs)) for c in (ctx, other)}
+    for j in jobs:
+        rows = max(k.pages for k in jobs) * 32
+        cache = [up(j.ctx, np.concatenate([y, np.zeros((rows - len(y), y.shape[1]), np.uint8)])) for y in j.cache]
+        b = own[id(j.ctx)]
+        b.set(j.new, j.start, j.table)
+        o = hip.HipBuffer.device_only(j.ctx, j.q.nbytes)
+        hip.enqueue_attention_paged(j.ctx, b, up(j.ctx, j.q), *cache, o)
+        outs.append(o)
+    got = [o.download(np.float16, j.q.shape) for o, j in zip(outs, jobs)]
+    for i in range(0, len(jobs), 2):
+        assert np.array_equal(got[i].view(np.uint16), got[i + 1].view(np.uint16))
+        check(got[i], *jobs[i].reference())
+    own[id(other)].release()
+    for j in jobs:
+        j.batch.release()
+    del outs, jobs
+    other.release()
 
 
 def test_two_batches_take_turns_without_a_wait(ctx):
@@ -469,6 +577,13 @@ def test_refusals(ctx):
     refused(bad, hip.enqueue_kv_store_paged, ctx, b, big, big2, big3, big4, small)
     refused(bad, hip.enqueue_kv_load_paged, ctx, b, big, big2, small, big4)
     refused(bad, hip.enqueue_kv_load_paged, ctx, b, big, big2, big3, big3)
+    for args in ((big, big2, big3, big2), (big, big2, big, big4), (big, big2, big3, big4, big2), (big, big2, big3, big4, big3),
+                 (big, big2, big3, big4, None, big), (big, big2, big3, big4, big, big)):  # one buffer twice
+        refused(bad, hip.enqueue_kv_store_paged, ctx, b, *args)
+    for args in ((big, big2, big, big4), (big, big2, big3, big2)):
+        refused(bad, hip.enqueue_kv_load_paged, ctx, b, *args)
+    for args in ((big, big2, big3, big2), (big, big2, big3, big3)):
+        refused(bad, hip.enqueue_attention_paged, ctx, b, *args)
     refused(bad, b.set, [1], [127], [[0] * 7 + [9]])
     hip.enqueue_attention_paged(ctx, b, big, big2, big3, big4)  # a refused set left the sequences as they were
     v = hip.SeqBatch(ctx)
@@ -480,26 +595,40 @@ def test_refusals(ctx):
                  (*ok[:4], 0, 1.0), (*ok[:4], 100, -1.0), (*ok[:4], 100, float("nan")), (*ok[:4], 100, float("inf"))):
         refused(bad, hip.enqueue_verify_drafts, ctx, v, *args, acc, ans)
     refused(bad, hip.enqueue_verify_drafts, ctx, v, *ok, acc, acc)
+    for x in (big, big2, big3, big4):
+        refused(bad, hip.enqueue_verify_drafts, ctx, v, *ok, x, ans)
+        refused(bad, hip.enqueue_verify_drafts, ctx, v, *ok, acc, x)
     refused(bad, hip.enqueue_attention_packed, ctx, v, big, big2, big3, big4)  # no head layout
     v.set([2, 0])
     refused(bad, hip.enqueue_verify_drafts, ctx, v, *ok, acc, ans)
     ctx.wait()
     b.release()
     b.release()
+    c = hip.SeqBatch(other, 4, 2, 64, 0, 16, 8)
+    h = c.handle
+    c.handle = type(h)()
+    hip.lib().sulimo_hip_seq_batch_release(h)
+    refused(bad, c.set, [1])
+    d = hip.SeqBatch(other, 4, 2, 64)
+    d.set([2])
+    d.release()
+    e = hip.SeqBatch(other)
+    e.release()
     other.release()
+    refused(bad, e.set, [1])  # its context is gone
 
 
 def test_empty_steps_do_nothing(ctx):
     b = hip.SeqBatch(ctx, 4, 2, 64, 0, 16, 8)
-    bufs = [up(ctx, np.full(8 * 16 * 136, 5, np.uint8)) for _ in range(4)]
+    bufs = [up(ctx, np.full(8 * 16 * 136, 5, np.uint8)) for _ in range(6)]
     for new, start in (([], []), ([0, 0], [0, 0])):
         b.set(new, start, np.zeros((len(new), 1), np.uint32))
-        hip.enqueue_kv_store_paged(ctx, b, *bufs)
-        hip.enqueue_kv_load_paged(ctx, b, *bufs)
-        hip.enqueue_attention_paged(ctx, b, *bufs)
+        hip.enqueue_kv_store_paged(ctx, b, *bufs[:4])
+        hip.enqueue_kv_load_paged(ctx, b, *bufs[:4])
+        hip.enqueue_attention_paged(ctx, b, *bufs[:4])
         b.set(new)
-        hip.enqueue_attention_packed(ctx, b, *bufs)
+        hip.enqueue_attention_packed(ctx, b, *bufs[:4])
         if not new:
-            hip.enqueue_verify_drafts(ctx, b, *bufs, 4, 1.0, bufs[0], bufs[2])
+            hip.enqueue_verify_drafts(ctx, b, *bufs[:4], 4, 1.0, *bufs[4:])
     for x in bufs:
         assert np.all(x.download(np.uint8, 8 * 16 * 136) == 5)

@@ -59,6 +59,21 @@ extern "C" void pieces(int heads, int kv_heads, int hd, int window, size_t n, co
   sizes[1] = (size_t)p.counters;
   sizes[2] = p.rec_rows;
 }
+// the pieces of a step's direct lists
+extern "C" void direct(int heads, int kv_heads, int hd, size_t n, const uint32_t *nn, const uint32_t *st, int32_t *out, size_t *sizes) {
+  SeqShape g{heads, kv_heads, hd, 0, 0, 0};
+  Seqs q;
+  plan_seqs(g, n, nn, st, nullptr, 0, &q);
+  std::vector<int> few, more;
+  for (size_t s = 0; s < n; s++) (q.n_new[s] * (heads / kv_heads) <= 16 ? few : more).push_back((int)s);
+  AttnPlan a[3];
+  plan_direct(g, q, few, more, 256, a);
+  for (int i = 0; i < 3; i++) {
+    sizes[i] = a[i].pieces.size();
+    memcpy(out, a[i].pieces.data(), sizes[i] * sizeof(AttnPiece));
+    out += 8 * sizes[i];
+  }
+}
 extern "C" uint32_t divided(uint32_t p, uint32_t d) {
   const FastDiv f = fast_div(d);
   return (uint32_t)(((uint64_t)p * f.magic) >> f.shift);
@@ -78,6 +93,7 @@ def lib(tmp_path_factory):
     L.shape_error.restype = L.plan.restype = C.c_char_p
     L.shape_error.argtypes = [C.c_size_t] * 6
     L.pieces.argtypes = [C.c_int] * 4 + [C.c_size_t] + [C.c_void_p] * 2 + [C.c_int] * 5 + [C.c_void_p] * 2
+    L.direct.argtypes = [C.c_int] * 3 + [C.c_size_t] + [C.c_void_p] * 4
     L.pieces.restype = None
     L.divided.argtypes, L.divided.restype = [C.c_uint32] * 2, C.c_uint32
     L.plan.argtypes = [C.c_int] * 3 + [C.c_size_t] + [C.c_void_p] * 3 + [C.c_size_t] + [C.c_void_p] * 2
@@ -223,6 +239,24 @@ def test_pieces_cover_every_key_once(lib, rows, key_tile, heads, sub, slots, win
             recs.append((ps[0][4], ps[0][4] + len(ps) * Hk * live))
     recs.sort()
     assert all(a[1] <= b[0] for a, b in zip(recs, recs[1:])) and (not recs or recs[-1][1] <= rec_rows)
+
+
+@pytest.mark.parametrize("new,start", [([1], [0]), ([1] * 64, [2000] * 64), ([8], [1000]), ([6] * 64, [2000] * 64),
+                                       ([1, 8] * 9, [500] * 18), ([5, 6] * 20, [4000] * 40), ([42, 1, 1], [9000, 10, 3]), ([], [])])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(24, 8, 128), (4, 2, 64), (5, 1, 128)])
+def test_direct_lists_cover_every_row_once(lib, heads, kv_heads, hd, new, start):
+    nn, st = np.asarray(new, np.uint32), np.asarray(start, np.uint32)
+    out, z = np.zeros(1 << 18, np.int32), np.zeros(3, np.uint64)
+    lib.direct(heads, kv_heads, hd, len(new), nn.ctypes.data, st.ctypes.data, out.ctypes.data, z.ctypes.data)
+    p, G, at, seen = out.reshape(-1, 8), heads // kv_heads, 0, set()
+    for rows, n in zip((16, 32, 0), (int(x) for x in z)):
+        tiles = {(int(seq), int(row0)) for seq, row0, *_ in p[at:at + n]}
+        at += n
+        assert rows or not n
+        for s in {t[0] for t in tiles}:
+            assert s not in seen and {t[1] for t in tiles if t[0] == s} == set(range(0, new[s] * G, rows))
+        seen |= {t[0] for t in tiles}
+    assert seen == set(range(len(new)))
 
 
 def test_division_by_the_page_size(lib):
