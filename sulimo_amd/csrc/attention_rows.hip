@@ -21,6 +21,13 @@
 // VALU leave the MFMA units busy 45 % of the time. Waves of 64 rows read half as much, but need
 // 485 registers and so stand alone on their SIMD: 542 us, the softmax's chains uncovered.
 //
+// EXACT, for keys read back from the Q8_0 cache: code * scale has up to 18 bits, so K and the
+// weights come in two f16 parts each, and only values and results are rounded, as where few rows
+// read the cache directly. One part each gave an rms error of 4.1e-4 of the result, two 2.9e-4
+// (rounding the result alone: 2.1e-4), for twice the MFMAs, half again the LDS reads and 333
+// registers, so that a workgroup of 128-wide heads has a CU alone: two chunks of 540 and 610 tokens
+// behind 4200 and 4600 positions 115 and 185 us.
+//
 // Keys and values that are not finite: a masked score is replaced before the softmax, but a
 // masked weight of 0 times such a value is not 0. A workgroup whose sums came out not finite
 // therefore runs once more, slowly, with such values taken out of the tiles that the mask
@@ -46,7 +53,7 @@ __device__ __forceinline__ void wait_vmcnt() {
 struct RowAttn {
   StepAttnArgs s;
   const SeqKv *kv;
-  const _Float16 *k, *v;
+  const _Float16 *k, *k_rest, *v;
 };
 
 // Chunk c of V row `row` stands at chunk c ^ vswz(row): the 4 rows x 64 bytes that 32 lanes of a
@@ -56,13 +63,15 @@ __device__ __forceinline__ int vswz(int row) {
   return HD == 128 ? 2 * (2 * (row & 3) + ((row >> 2) & 1)) : 2 * (2 * ((row >> 1) & 1) + ((row >> 2) & 1));
 }
 
-template <int HD>
-__global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
+template <int HD, bool EXACT>
+__global__ __launch_bounds__(256, EXACT && HD == 128 ? 1 : 2) void row_attn_kernel(RowAttn a) {
   constexpr int KS = HD / 16, OT = HD / 32, KCH = HD / 8;
   constexpr int ROWB = HD * 2, TILE = kRowKeys * ROWB;
   constexpr int RPI = 64 / KCH;             // rows per DMA instruction
   constexpr int NI = kRowKeys / RPI / 4;    // DMA instructions per wave and tile
-  __shared__ __attribute__((aligned(16))) char ka[TILE], va[TILE], kb[TILE], vb[TILE];
+  constexpr int REST = EXACT ? TILE : 16;
+  constexpr int NK = EXACT ? 2 * NI : NI;   // of a K tile
+  __shared__ __attribute__((aligned(16))) char ka[TILE], va[TILE], kb[TILE], vb[TILE], ra[REST], rb[REST];
   __shared__ int shared_flag;
   const int n_head_kv = a.s.n_head_kv, n_head = a.s.n_head, G = n_head / n_head_kv;
   const int kvh = blockIdx.x % n_head_kv;
@@ -96,6 +105,8 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
   const uint32_t bytes = (uint32_t)(kv.len - 1) * stride + ROWB;
   const rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<_Float16 *>(a.k + base), (short)0, (int)bytes, (int)kRsrcWord3);
   const rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<_Float16 *>(a.v + base), (short)0, (int)bytes, (int)kRsrcWord3);
+  const rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc(const_cast<_Float16 *>(EXACT ? a.k_rest + base : nullptr), (short)0,
+                                                      EXACT ? (int)bytes : 0, (int)kRsrcWord3);
   uint32_t koff[NI], voff[NI];
 #pragma unroll
   for (int i = 0; i < NI; i++) {
@@ -110,6 +121,20 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
     for (int i = 0; i < NI; i++) dma16(rs, dst + RPI * (NI * wave + i) * ROWB, o[i] + so, 0);
   };
 
+  // K of a tile, and with EXACT what its rounding dropped
+  struct KTile {
+    char *k, *rest;
+  };
+  const KTile slot_a{ka, ra}, slot_b{kb, rb};
+  auto issue_k = [&](const KTile &dst, int tile) __attribute__((always_inline)) {
+    issue(rk, koff, dst.k, tile);
+    if constexpr (EXACT) issue(rr, koff, dst.rest, tile);
+  };
+  // Weights of a half tile in f16, and with EXACT what that rounding dropped
+  struct Weights {
+    half8 p[2], rest[EXACT ? 2 : 1];
+  };
+
   floatx16 o[OT];
   float mrun, lrun;
   auto reset = [&]() {
@@ -119,10 +144,11 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
     lrun = 0.0f;
   };
 
-  auto s_mfma = [&](const char *sk, int kt, int s, floatx16 &st) __attribute__((always_inline)) {
-    const int row = 32 * kt + l32;
-    const half8 kf = *reinterpret_cast<const half8 *>(sk + row * ROWB + 16 * ((2 * s + lg) ^ (row % KCH)));
-    st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], st, 0, 0, 0);
+  auto s_mfma = [&](const KTile &sk, int kt, int s, floatx16 &st) __attribute__((always_inline)) {
+    const int row = 32 * kt + l32, at = row * ROWB + 16 * ((2 * s + lg) ^ (row % KCH));
+    st = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8 *>(sk.k + at), qf[s], st, 0, 0, 0);
+    if constexpr (EXACT)
+      st = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8 *>(sk.rest + at), qf[s], st, 0, 0, 0);
   };
   // V^T fragment of dimensions 32 i .. and keys 32 kt + 16 j + {0-3, 8-11} + 4 lg
   const int vr = 4 * lg + ((lane & 15) >> 2), vc = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), vb8 = 8 * (lane & 1);
@@ -134,9 +160,12 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
     const char *p = sv + (32 * kt + 16 * j) * ROWB, *q = p + 8 * ROWB;
     return read_tr(p + lane_at, q + lane_at);
   };
-  auto pv_mfma = [&](const char *sv, int kt, int s, const half8 (&pp)[2]) __attribute__((always_inline)) {
-    const int j = s / OT, i = s % OT;
-    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(sv, kt, j, i), pp[j], o[i], 0, 0, 0);
+  auto add_values = [&](const half8 &vf, int j, int i, const Weights &w) __attribute__((always_inline)) {
+    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w.p[j], o[i], 0, 0, 0);
+    if constexpr (EXACT) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w.rest[j], o[i], 0, 0, 0);
+  };
+  auto pv_mfma = [&](const char *sv, int kt, int s, const Weights &w) __attribute__((always_inline)) {
+    add_values(v_frag(sv, kt, s / OT, s % OT), s / OT, s % OT, w);
   };
   static_assert(2 * OT == KS, "a half tile's S and PV take equally many MFMAs");
   auto mask = [&](floatx16 &st, int p_reg0) __attribute__((always_inline)) {
@@ -146,7 +175,7 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
       st[e] = (p > P || p <= P - win) ? -INFINITY : st[e];
     }
   };
-  auto softmax = [&](const floatx16 &st, half8 (&pb)[2]) __attribute__((always_inline)) -> float {
+  auto softmax = [&](const floatx16 &st, Weights &w) __attribute__((always_inline)) -> float {
     float mt = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; e++) mt = fmaxf(mt, st[e]);
@@ -155,12 +184,23 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
     const float alpha = grow && mrun != -INFINITY ? __builtin_amdgcn_exp2f(mrun - mt) : 1.0f;
     if (grow) mrun = mt;
     const float ms = mrun == -INFINITY ? 0.0f : mrun;
-#pragma unroll
-    for (int e = 0; e < 16; e++) pb[e >> 3][e & 7] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[e], c, -ms));
-    const half2v one = {(_Float16)1.0f, (_Float16)1.0f};
     float sum = 0.0f;
+    if constexpr (EXACT) {
 #pragma unroll
-    for (int e = 0; e < 16; e += 2) sum = __builtin_amdgcn_fdot2(half2v{pb[e >> 3][e & 7], pb[e >> 3][(e & 7) + 1]}, one, sum, false);
+      for (int e = 0; e < 16; e++) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e], c, -ms));
+        const _Float16 hi = (_Float16)x;
+        w.p[e >> 3][e & 7] = hi;
+        w.rest[e >> 3][e & 7] = (_Float16)(x - (float)hi);
+        sum += x;
+      }
+    } else {  // the sum of the weights as they are rounded: their common error cancels
+#pragma unroll
+      for (int e = 0; e < 16; e++) w.p[e >> 3][e & 7] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[e], c, -ms));
+      const half2v one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) sum = __builtin_amdgcn_fdot2(half2v{w.p[e >> 3][e & 7], w.p[e >> 3][(e & 7) + 1]}, one, sum, false);
+    }
     lrun = lrun * alpha + sum;
     return alpha;
   };
@@ -171,8 +211,8 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
     }
   };
   // The S^T MFMAs of half tile h+1 and the PV MFMAs of h-1 under the softmax of h.
-  auto phase = [&](const char *sk, int kt, floatx16 &snext, const char *sv, int vt, const half8 (&pp)[2],
-                   const floatx16 &scur, half8 (&pc_)[2]) __attribute__((always_inline)) {
+  auto phase = [&](const KTile &sk, int kt, floatx16 &snext, const char *sv, int vt, const Weights &pp,
+                   const floatx16 &scur, Weights &pc_) __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
     snext = floatx16{};
 #pragma unroll
@@ -181,16 +221,19 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
       pv_mfma(sv, vt, s, pp);
     }
     const float alpha = softmax(scur, pc_);
-    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+    // LDS reads two pairs of steps ahead (1 of K, or 2, and 2 of V), the softmax's VALU between
+    __builtin_amdgcn_sched_group_barrier(0x100, EXACT ? 8 : 6, 0);
 #pragma unroll
     for (int k = 0; k < 2 * KS; k++) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                              // 1 MFMA
-      if (k + 4 < 2 * KS) {  // LDS reads two pairs ahead: 1 of K, 2 of V
-        if (k & 1) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, EXACT ? 2 : 1, 0);  // MFMA
+      if (k + 4 < 2 * KS) {
+        if (EXACT || (k & 1)) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);                              // 5 VALU
+      __builtin_amdgcn_sched_group_barrier(0x002, EXACT ? 8 : 5, 0);  // VALU
     }
+    if constexpr (EXACT)  // the compiler would move this phase's exponentials behind the next one's MFMAs
+      asm volatile("" : "+v"(pc_.p[0]), "+v"(pc_.p[1]), "+v"(pc_.rest[0]), "+v"(pc_.rest[1]), "+v"(lrun));
     __builtin_amdgcn_sched_barrier(0);
     rescale(alpha);
   };
@@ -203,8 +246,8 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
 
   auto fast = [&]() __attribute__((always_inline)) {
     floatx16 sa, sb;
-    half8 pa[2], pb[2];
-    auto first = [&](const char *sk, int tile) __attribute__((always_inline)) {  // S^T of both halves, P of the first
+    Weights pa, pb;
+    auto first = [&](const KTile &sk, int tile) __attribute__((always_inline)) {  // S^T of both halves, P of the first
       sa = floatx16{};
       sb = floatx16{};
 #pragma unroll
@@ -222,7 +265,7 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
 #pragma unroll
       for (int s = 0; s < KS; s++) pv_mfma(sv, 1, s, pb);
     };
-    auto both = [&](const char *sk, const char *sv, int tile) __attribute__((always_inline)) {
+    auto both = [&](const KTile &sk, const char *sv, int tile) __attribute__((always_inline)) {
       const int p1 = tile * kRowKeys + 32 + 4 * lg;
       if (!unmasked(tile)) mask(sb, p1);
       phase(sk, 0, sa, sv, 0, pa, sb, pb);
@@ -231,12 +274,12 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
     };
     // At the start of step t the K tile of t + 1 and the V tile of t have landed, and every wave
     // is done with the slots that K of t + 2 and V of t + 1 go to.
-    auto step = [&](char *k_use, char *k_next, char *v_use, char *v_next, int u) __attribute__((always_inline)) {
+    auto step = [&](const KTile &k_use, const KTile &k_next, char *v_use, char *v_next, int u) __attribute__((always_inline)) {
       __builtin_amdgcn_sched_barrier(0);
       wait_vmcnt<0>();
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
-      if (u + 2 < steps) issue(rk, koff, k_next, tb + u + 2);
+      if (u + 2 < steps) issue_k(k_next, tb + u + 2);
       if (u + 1 < steps) issue(rv, voff, v_next, tb + u + 1);
       const int tile = tb + u;
       const bool more = u + 1 < steps && visible(tile + 1);
@@ -247,19 +290,18 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
         if (more) first(k_use, tile + 1);
       }
     };
-    issue(rk, koff, ka, tb);  // first: the wait below counts on all others being younger
+    issue_k(slot_a, tb);  // first: the wait below counts on all others being younger
     __builtin_amdgcn_sched_barrier(0);
     issue(rv, voff, va, tb);
-    if (steps > 1) issue(rk, koff, kb, tb + 1);
-    else issue(rk, koff, kb, tb);
+    issue_k(slot_b, steps > 1 ? tb + 1 : tb);
     __builtin_amdgcn_sched_barrier(0);
-    wait_vmcnt<2 * NI>();
+    wait_vmcnt<NI + NK>();
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    if (visible(tb)) first(ka, tb);
+    if (visible(tb)) first(slot_a, tb);
     for (int u = 0; u < steps; u += 2) {
-      step(kb, ka, va, vb, u);
-      if (u + 1 < steps) step(ka, kb, vb, va, u + 1);
+      step(slot_b, slot_a, va, vb, u);
+      if (u + 1 < steps) step(slot_a, slot_b, vb, va, u + 1);
     }
     wait_vmcnt<0>();
     __syncthreads();
@@ -269,7 +311,7 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
   auto careful = [&]() {
     for (int u = 0; u < steps; u++) {
       const int tile = tb + u;
-      issue(rk, koff, ka, tile);
+      issue_k(slot_a, tile);
       issue(rv, voff, va, tile);
       wait_vmcnt<0>();
       __syncthreads();
@@ -279,10 +321,11 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
         for (int kt = 0; kt < 2; kt++) {
           floatx16 st{};
 #pragma unroll
-          for (int s = 0; s < KS; s++) s_mfma(ka, kt, s, st);
+          for (int s = 0; s < KS; s++) s_mfma(slot_a, kt, s, st);
           const int p0 = tile * kRowKeys + 32 * kt + 4 * lg;
           if (crossed) mask(st, p0);
-          half8 pp[2], seen[2];
+          Weights pp;
+          half8 seen[2];
 #pragma unroll
           for (int e = 0; e < 16; e++) {
             const int p = p0 + 8 * (e >> 2) + (e & 3);
@@ -306,7 +349,7 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
               nn[e] = x && (b & 0x3ffu) ? (_Float16)1.0f : (_Float16)0.0f;
               vf[e] = x ? (_Float16)0.0f : vf[e];
             }
-            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pp[j], o[i], 0, 0, 0);
+            add_values(vf, j, i, pp);
             if (__ballot(odd)) {
               const floatx16 u1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(up, seen[j], floatx16{}, 0, 0, 0);
               const floatx16 d1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(dn, seen[j], floatx16{}, 0, 0, 0);
@@ -376,11 +419,14 @@ __global__ __launch_bounds__(256, 2) void row_attn_kernel(RowAttn a) {
 
 }  // namespace
 
-int32_t launch_row_attention(const StepAttnArgs &c, const SeqKv *kv, const _Float16 *k, const _Float16 *v, hipStream_t s) {
-  RowAttn a{c, kv, k, v};
-  const dim3 grid((unsigned)c.n_pieces * c.n_head_kv);
-  if (c.head_dim == 64) hipLaunchKernelGGL((row_attn_kernel<64>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((row_attn_kernel<128>), grid, dim3(256), 0, s, a);
+int32_t launch_row_attention(const StepAttnArgs &c, const SeqKv *kv, const _Float16 *k, const _Float16 *k_rest,
+                             const _Float16 *v, hipStream_t s) {
+  RowAttn a{c, kv, k, k_rest, v};
+  const dim3 grid((unsigned)c.n_pieces * c.n_head_kv), block(256);
+  if (c.head_dim == 64 && k_rest) hipLaunchKernelGGL((row_attn_kernel<64, true>), grid, block, 0, s, a);
+  else if (c.head_dim == 64) hipLaunchKernelGGL((row_attn_kernel<64, false>), grid, block, 0, s, a);
+  else if (k_rest) hipLaunchKernelGGL((row_attn_kernel<128, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((row_attn_kernel<128, false>), grid, block, 0, s, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? SULIMO_HIP_OK : hip_fail(e, "row_attn_kernel launch");
 }

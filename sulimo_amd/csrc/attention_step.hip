@@ -19,10 +19,12 @@ namespace {
 constexpr size_t align_up(size_t v) { return (v + 255) & ~(size_t)255; }
 
 // Rows a KV head up to which a sequence's rows read the Q8_0 cache directly; more have it read
-// back and go to the row kernel. Measured, 24 heads over 8, directly and by read-back: 126 rows of
-// one sequence behind 8000 positions 31 and 58 us, of 16 behind 4000 151 and 178, of 64 behind
-// 2000 288 and 296; 192 rows 43 and 57, 218 and 180, 479 and 407.
-constexpr int kDirectRows = 128;
+// back and go to the row kernel. Measured, 24 heads over 8, directly and by read-back: 192 rows of
+// one sequence behind 8000 positions 44 and 73 us, of 16 behind 4000 229 and 277, of 64 behind
+// 2000 486 and 621; 255 rows 50 and 77, 281 and 289, 697 and 645; 384 rows of one 72 and 76, of
+// 16 behind 1000 133 and 118, behind 4000 434 and 435; 768 rows 126 and 99, 245 and 188, 971 and
+// 652.
+constexpr int kDirectRows = 256;
 
 int32_t plan(sulimo_hip_seq_batch *b, bool packed) {
   StepPlan &p = packed ? b->packed_plan : b->paged_plan;
@@ -35,7 +37,7 @@ int32_t plan(sulimo_hip_seq_batch *b, bool packed) {
   }
   AttnPlan a[3];
   plan_direct(b->g, b->q, which[0], which[1], cus, a);
-  a[2] = plan_attention_pieces(b->g, b->q, which[2], row_split(cus));
+  a[2] = plan_attention_pieces(b->g, b->q, which[2], row_split(b->g, !packed, cus));
   std::vector<SeqKv> kv(b->q.n_seqs, SeqKv{0, 0, 0});
   std::vector<LoadTile> tiles;
   long rows = 0;
@@ -85,7 +87,7 @@ int32_t attend(sulimo_hip_seq_batch *b, StepPlan &p, const uint16_t *q, const ui
   const size_t hd = b->g.head_dim, width = (size_t)b->g.n_head_kv * hd;
   const size_t o_bytes = align_up(p.rec_rows * hd * 4), ml_bytes = align_up(p.rec_rows * 8);
   const size_t kv_bytes = align_up((size_t)p.read_rows * width * 2);
-  STEP_TRY(ensure_workspace(ctx, o_bytes + ml_bytes + 2 * kv_bytes));
+  STEP_TRY(ensure_workspace(ctx, o_bytes + ml_bytes + 3 * kv_bytes));
   char *ws = reinterpret_cast<char *>(ctx->ws), *lists = reinterpret_cast<char *>(p.lists.dev);
   auto args = [&](const StepPlan::List &l) {
     return StepAttnArgs{seq_view(b), reinterpret_cast<const AttnPiece *>(lists + l.at), l.n,
@@ -97,15 +99,18 @@ int32_t attend(sulimo_hip_seq_batch *b, StepPlan &p, const uint16_t *q, const ui
   for (int i = 0; i < 2; i++)
     if (p.list[i].n) STEP_TRY(launch_cache_attention(args(p.list[i]), i + 1, k_cache, v_cache, ctx->stream));
   if (p.list[2].n) {
+    uint16_t *k_rest = nullptr;
     if (p.n_tiles) {
       uint16_t *kr = reinterpret_cast<uint16_t *>(ws + o_bytes + ml_bytes), *vr = kr + kv_bytes / 2;
+      k_rest = vr + kv_bytes / 2;
       STEP_TRY(launch_kv_load_paged(reinterpret_cast<const LoadTile *>(lists + p.at_tiles), p.n_tiles, seq_view(b).pages,
-                                    b->g.page_size, (int)width, k_cache, v_cache, kr, vr, ctx->stream));
+                                    b->g.page_size, (int)width, k_cache, v_cache, kr, vr, k_rest, ctx->stream));
       k = kr;
       v = vr;
     }
     STEP_TRY(launch_row_attention(args(p.list[2]), reinterpret_cast<const SeqKv *>(lists + p.at_kv),
-                                  reinterpret_cast<const _Float16 *>(k), reinterpret_cast<const _Float16 *>(v), ctx->stream));
+                                  reinterpret_cast<const _Float16 *>(k), reinterpret_cast<const _Float16 *>(k_rest),
+                                  reinterpret_cast<const _Float16 *>(v), ctx->stream));
   }
   return SULIMO_HIP_OK;
 }

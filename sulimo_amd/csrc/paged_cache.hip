@@ -97,12 +97,12 @@ __global__ __launch_bounds__(256) void kv_store_paged_kernel(const int32_t *row_
 // look-up, read 12 conversations of 2000 to 8000 positions at 4.0 TB/s).
 __global__ __launch_bounds__(256) void kv_load_paged_kernel(const LoadTile *tiles, const int32_t *pages, int page_size,
                                                             int width, const uint8_t *k_cache, const uint8_t *v_cache,
-                                                            _Float16 *k_out, _Float16 *v_out) {
+                                                            _Float16 *k_out, _Float16 *v_out, _Float16 *k_rest) {
   __shared__ uint32_t slots[kLoadTile];
   constexpr int kDeep = 4;
   const LoadTile t = tiles[blockIdx.x];
   const uint8_t *cache = blockIdx.y ? v_cache : k_cache;
-  _Float16 *out = blockIdx.y ? v_out : k_out;
+  _Float16 *out = blockIdx.y ? v_out : k_out, *rest = blockIdx.y ? nullptr : k_rest;
   if ((int)threadIdx.x < t.count) {
     const uint32_t p = (uint32_t)t.pos + threadIdx.x, pg = p / (uint32_t)page_size;
     slots[threadIdx.x] = (uint32_t)pages[t.page_off + pg] * (uint32_t)page_size + (p - pg * (uint32_t)page_size);
@@ -150,13 +150,23 @@ __global__ __launch_bounds__(256) void kv_load_paged_kernel(const LoadTile *tile
 #pragma unroll
         for (int i = 0; i < 4; i++) c[i] = w[e][i];
       }
-      half8 o[2];
+      half8 o[2], low[2];
 #pragma unroll
-      for (int i = 0; i < 16; i++) o[i >> 3][i & 7] = (_Float16)((float)(int8_t)(c[i >> 2] >> (8 * (i & 3))) * d);
+      for (int i = 0; i < 16; i++) {
+        const float x = (float)(int8_t)(c[i >> 2] >> (8 * (i & 3))) * d;
+        const _Float16 hi = (_Float16)x;
+        o[i >> 3][i & 7] = hi;
+        low[i >> 3][i & 7] = fabsf((float)hi) < INFINITY ? (_Float16)(x - (float)hi) : (_Float16)0.0f;
+      }
       if (r[e] < count) {
         _Float16 *y = out + ((size_t)t.out_row + r[e]) * width + pt[e] * 16;
         *reinterpret_cast<half8 *>(y) = o[0];
         *reinterpret_cast<half8 *>(y + 8) = o[1];
+        if (rest) {
+          _Float16 *z = rest + (y - out);
+          *reinterpret_cast<half8 *>(z) = low[0];
+          *reinterpret_cast<half8 *>(z + 8) = low[1];
+        }
       }
     }
   }
@@ -180,9 +190,10 @@ int32_t launch_kv_store_paged(const SeqView &v, int width, const uint16_t *k, co
 
 int32_t launch_kv_load_paged(const LoadTile *tiles, int n_tiles, const int32_t *pages, int page_size, int width,
                              const uint8_t *k_cache, const uint8_t *v_cache, uint16_t *k_out, uint16_t *v_out,
-                             hipStream_t s) {
+                             uint16_t *k_rest, hipStream_t s) {
   hipLaunchKernelGGL(kv_load_paged_kernel, dim3(n_tiles, 2), dim3(256), 0, s, tiles, pages, page_size, width, k_cache,
-                     v_cache, reinterpret_cast<_Float16 *>(k_out), reinterpret_cast<_Float16 *>(v_out));
+                     v_cache, reinterpret_cast<_Float16 *>(k_out), reinterpret_cast<_Float16 *>(v_out),
+                     reinterpret_cast<_Float16 *>(k_rest));
   return launched("kv_load_paged_kernel");
 }
 

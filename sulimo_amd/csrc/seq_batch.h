@@ -58,9 +58,10 @@ int32_t step_array(sulimo_hip_seq_batch *b, StepArray *a, size_t bytes);
 // Kernel launchers of a step's operators.
 int32_t launch_kv_store_paged(const SeqView &v, int width, const uint16_t *k, const uint16_t *vv, uint8_t *k_cache,
                               uint8_t *v_cache, uint16_t *k_values, uint16_t *v_values, hipStream_t s);
+// k_rest: what the rounding of k_out to f16 dropped, or null.
 int32_t launch_kv_load_paged(const LoadTile *tiles, int n_tiles, const int32_t *pages, int page_size, int width,
                              const uint8_t *k_cache, const uint8_t *v_cache, uint16_t *k_out, uint16_t *v_out,
-                             hipStream_t s);
+                             uint16_t *k_rest, hipStream_t s);
 
 // Attention of the batch's new rows: over the paged Q8_0 cache (k_cache, v_cache bytes), or
 // over the rows' own f16 keys and values.

@@ -210,7 +210,8 @@ int32_t sulimo_hip_enqueue_kv_load_paged(sulimo_hip_ctx *ctx, sulimo_hip_seq_bat
     wrote(v_out);
     return launch_kv_load_paged(reinterpret_cast<const LoadTile *>(b->load_tiles.dev), b->n_load_tiles,
                                 seq_view(b).pages, b->g.page_size, (int)row_width(b), dp<const uint8_t>(k_cache),
-                                dp<const uint8_t>(v_cache), dp<uint16_t>(k_out), dp<uint16_t>(v_out), ctx->stream);
+                                dp<const uint8_t>(v_cache), dp<uint16_t>(k_out), dp<uint16_t>(v_out), nullptr,
+                                ctx->stream);
   });
 }
 

@@ -328,7 +328,12 @@ inline void plan_direct(const SeqShape &g, const Seqs &q, const std::vector<int>
 // 206, the eight prompts of 677 to 4000 tokens 285 and 420. A tile is cut where a chunk is short
 // and its history long.
 constexpr int kRowTile = 128, kRowKeys = 64;
-inline AttnSplit row_split(int cus) { return AttnSplit{kRowTile, kRowKeys, 1, 1, 2 * cus, 256, 4.0, 24.0, 2.1, 1.2, 1.8}; }
+// exact: keys and weights in two f16 parts each, for which a workgroup of 128-wide heads takes a
+// CU's registers alone.
+inline AttnSplit row_split(const SeqShape &g, bool exact, int cus) {
+  if (exact && g.head_dim == 128) return AttnSplit{kRowTile, kRowKeys, 1, 1, cus, 256, 4.0, 24.0, 2.3, 2.3, 1.8};
+  return AttnSplit{kRowTile, kRowKeys, 1, 1, 2 * cus, 256, 4.0, 24.0, 2.1, 1.2, 1.8};
+}
 
 // Where a sequence's f16 keys and values lie: position p in [lo, lo + len) is row row0 + p - lo.
 struct SeqKv {

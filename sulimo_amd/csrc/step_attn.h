@@ -27,8 +27,10 @@ struct StepAttnArgs {
   Join join;
 };
 int32_t launch_cache_attention(const StepAttnArgs &c, int row_tiles, const uint8_t *k_cache, const uint8_t *v_cache, hipStream_t s);
-// kv: where each sequence's f16 keys and values lie in k and v ([rows][n_head_kv][head_dim])
-int32_t launch_row_attention(const StepAttnArgs &c, const SeqKv *kv, const _Float16 *k, const _Float16 *v, hipStream_t s);
+// kv: where each sequence's f16 keys and values lie in k and v ([rows][n_head_kv][head_dim]).
+// k_rest: what the keys' rounding to f16 dropped, or null: the keys are f16 numbers.
+int32_t launch_row_attention(const StepAttnArgs &c, const SeqKv *kv, const _Float16 *k, const _Float16 *k_rest,
+                             const _Float16 *v, hipStream_t s);
 
 namespace {
 

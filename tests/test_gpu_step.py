@@ -202,6 +202,7 @@ STEPS = [
     ([700, 3, 0, 129], [1, 5, 1, 2], 32, 0), ([10, 0, 5], [0, 3, 0], 16, 0), ([0], [33], 16, 0), ([5], [70], 100, 0),
     ([400, 2], [40, 1], 64, 0), ([0, 190], [130, 64], 1, 0), ([90], [200], 256, 0),
     ([500], [1], 16, 1), ([500, 20], [1, 4], 16, 33), ([300], [50], 32, 64), ([0, 77], [90, 1], 16, 40), ([200], [9], 16, 4000),
+    ([300], [270], 32, 64), ([500, 3, 90], [300, 1, 5], 16, 0),
 ]
 
 
@@ -229,10 +230,27 @@ def test_attention_paged_repeats_bit_for_bit(ctx):
     assert np.array_equal(a.view(np.uint16), b.view(np.uint16))
 
 
+@pytest.mark.parametrize("heads", [(24, 8, 128), (4, 2, 64)])
+def test_a_chunk_is_as_near_as_its_tokens_alone(ctx, heads):
+    """A chunk whose part of the cache is read back, and the same rows eight at a time, which read it
+    directly: both round values and results to f16 and nothing else, so their errors are alike."""
+    start, n = 700, 320
+    st = Step(ctx, np.random.default_rng(36), heads, [start], [n], 64, 0, spikes=False)
+    want, _ = st.reference()
+    whole = st.attend()[:n]
+    q, parts = st.q, []
+    for t in range(0, n, 8):
+        st.batch.set([8], [start + t], st.table)
+        st.q, st.rows = q[t:t + 8], 8
+        parts.append(st.attend()[:8])
+    rms = [np.sqrt(np.mean((x.astype(np.float64) - want) ** 2)) for x in (whole, np.concatenate(parts))]
+    assert rms[0] <= 1.2 * rms[1] and rms[1] <= 1.2 * rms[0]
+
+
 def test_attention_hides_what_is_not_finite(ctx):
     """A later token's keys and values that are NaN or infinite stay out of earlier tokens' sums."""
     for heads in [(12, 2, 128), (4, 2, 64)]:
-        for start, n in (([40], 6), ([20], 100)):
+        for start, n in (([40], 6), ([20], 100), ([20], 300)):
             st = Step(ctx, np.random.default_rng(9), heads, start, [n], 16, 0, spikes=False)
             bad = R.slots(st.table[0], 16, start[0] + n - 1, start[0] + n)
             for w, code in ((0, np.nan), (1, np.inf)):
