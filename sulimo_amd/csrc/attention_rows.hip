@@ -225,12 +225,16 @@ __global__ __launch_bounds__(256, EXACT && HD == 128 ? 1 : 2) void row_attn_kern
     __builtin_amdgcn_sched_group_barrier(0x100, EXACT ? 8 : 6, 0);
 #pragma unroll
     for (int k = 0; k < 2 * KS; k++) {
-      __builtin_amdgcn_sched_group_barrier(0x008, EXACT ? 2 : 1, 0);  // MFMA
+      if (EXACT) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
       if (k + 4 < 2 * KS) {
         if (EXACT || (k & 1)) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x002, EXACT ? 8 : 5, 0);  // VALU
+      __builtin_amdgcn_sched_group_barrier(0x002, EXACT ? 4 : 5, 0);  // VALU
     }
     if constexpr (EXACT)  // the compiler would move this phase's exponentials behind the next one's MFMAs
       asm volatile("" : "+v"(pc_.p[0]), "+v"(pc_.p[1]), "+v"(pc_.rest[0]), "+v"(pc_.rest[1]), "+v"(lrun));
