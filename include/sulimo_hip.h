@@ -393,7 +393,9 @@ int32_t sulimo_hip_enqueue_kv_load_paged(sulimo_hip_ctx *ctx, sulimo_hip_seq_bat
                                          sulimo_hip_buffer *k_out, sulimo_hip_buffer *v_out);
 /* Causal GQA attention of the new rows over the paged cache (their own keys and values
  * stored before, sulimo_hip_enqueue_kv_store_paged): q, out f16 [rows][head_count][head_dim];
- * scores scaled by 1/sqrt(head_dim), softmax and sums in f32. */
+ * scores scaled by 1/sqrt(head_dim), softmax and sums in f32. Sequences of more than 256 new
+ * rows a KV head (n_new * head_count / head_count_kv) take 6 bytes of the context's workspace
+ * for every cached key element in their sight. */
 int32_t sulimo_hip_enqueue_attention_paged(sulimo_hip_ctx *ctx, sulimo_hip_seq_batch *batch,
                                            const sulimo_hip_buffer *q, const sulimo_hip_buffer *k_cache,
                                            const sulimo_hip_buffer *v_cache, sulimo_hip_buffer *out);

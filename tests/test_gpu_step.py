@@ -262,12 +262,13 @@ def test_attention_hides_what_is_not_finite(ctx):
             assert not np.any(np.isfinite(got[n - 1]))
 
 
-def test_a_cache_past_four_gigabytes(ctx):
+@pytest.mark.parametrize("page,pages", [(64, 64000), (48, 84000)])
+def test_a_cache_past_four_gigabytes(ctx, page, pages):
     """Pages whose bytes lie past 2^32 hold and give what those at the front do, for single tokens, a
     short chunk and one that is read back."""
     rng = np.random.default_rng(33)
-    H, Hk, hd, page, pages = 24, 8, 128, 64, 64000
-    width, S = Hk * hd, 3
+    H, Hk, hd = 24, 8, 128
+    width, each = Hk * hd, -(-333 // page)
     assert pages * page * (width // 32) * 34 > 1 << 32
     start, new = [0, 0, 0], [260, 300, 333]
     k, v = (randn16(rng, sum(new), width) for _ in range(2))
@@ -276,8 +277,8 @@ def test_a_cache_past_four_gigabytes(ctx):
     q = [randn16(rng, sum(n), H, hd) for _, n in steps]
     cache = [hip.HipBuffer.device_only(ctx, pages * page * (width // 32) * 34) for _ in range(2)]
     answers = []
-    for first in (0, pages - 18):
-        table = first + np.arange(18, dtype=np.uint32).reshape(3, 6)[:, ::-1]
+    for first in (0, pages - 3 * each):
+        table = first + np.arange(3 * each, dtype=np.uint32).reshape(3, each)[:, ::-1]
         batch = hip.SeqBatch(ctx, H, Hk, hd, 0, page, pages)
         batch.set(new, start, table)
         hip.enqueue_kv_store_paged(ctx, batch, *kv, *cache)
@@ -311,6 +312,35 @@ def test_pages_behind_the_window_may_stand_for_anything(ctx, new):
     x.batch.set(x.new, x.start, table)
     assert np.array_equal(x.attend().view(np.uint16), want.view(np.uint16))
     check(want[:-3], *x.reference())
+
+
+def test_prefills_and_steps_in_turn(ctx):
+    """A prefill of one sequence and steps of several share the context's workspace, and neither
+    changes what the other gives."""
+    from sulimo_amd import synthetic as S
+    cfg = S.ModelConfig(2, 256, 512, 4, 2, 64, 64, 512, 1e6, 1e-6, 1)
+    dm = hip.DeviceModel(ctx, S.make_model(cfg, 7), capacity=64, max_n=16)
+    toks = S.random_tokens(8, 32, cfg.vocab)
+    steps = [Step(ctx, np.random.default_rng([37, i]), (4, 2, 64), start, new, 16) for i, (start, new) in
+             enumerate([([900], [1]), ([50, 700], [300, 4]), ([2000] * 30, [9] * 30)])]
+    alone = [x.attend() for x in steps]
+
+    def prefill(between):
+        out = []
+        for at in (0, 16):
+            dm.embed(toks[at:at + 16])
+            dm.execute_prefill_ubatch(at, 16)
+            out.append(dm.logits().copy())
+            between(at)
+        return out
+
+    want = prefill(lambda at: None)
+    for turn in range(3):
+        got = []
+        logits = prefill(lambda at: got.extend(x.attend() for x in steps))
+        assert all(np.array_equal(a, b) for a, b in zip(logits, want)), turn
+        assert all(np.array_equal(a.view(np.uint16), b.view(np.uint16)) for a, b in zip(got, alone + alone)), turn
+    dm.release()
 
 
 def test_contexts_and_batches_that_grow_and_shrink(ctx):
