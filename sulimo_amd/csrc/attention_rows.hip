@@ -26,7 +26,8 @@
 // read the cache directly. One part each gave an rms error of 4.1e-4 of the result, two 2.9e-4
 // (rounding the result alone: 2.1e-4), for twice the MFMAs, half again the LDS reads and 333
 // registers, so that a workgroup of 128-wide heads has a CU alone: two chunks of 540 and 610 tokens
-// behind 4200 and 4600 positions 115 and 185 us.
+// behind 4200 and 4600 positions 115 and 178 us. Eight waves, each half of every key tile, spill
+// their registers: 195.
 //
 // Keys and values that are not finite: a masked score is replaced before the softmax, but a
 // masked weight of 0 times such a value is not 0. A workgroup whose sums came out not finite
